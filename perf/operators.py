@@ -238,6 +238,11 @@ def prepare(case, seed):
 
 
 # ---------------------------------------------------------------- the plain forms
+def _over(x, n):
+    """x / n, correctly rounded (a Python number as divisor becomes a product with its reciprocal on the GPU)."""
+    return x / torch.full((), n, dtype=x.dtype, device=x.device)
+
+
 def _groups(case, x):
     return x.reshape(*x.shape[:-1], case["head_dim"] // case["group"], case["group"])
 
@@ -247,12 +252,12 @@ def _quantize(case, x):
     if case["bits"] == 8:
         g = _groups(case, x)
         lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-        scale = ((hi.float() - lo.float()).to(x.dtype).float() / 255.0).clamp_min(1e-8)
+        scale = _over((hi.float() - lo.float()).to(x.dtype).float(), 255.0).clamp_min(1e-8)
         codes = ((g.float() - lo.float()).to(x.dtype).float() / scale).clamp(0.0, 255.0).trunc()
         return codes.to(torch.uint8).reshape(x.shape), scale[..., 0].half(), lo[..., 0].half()
     g = _groups(case, torch.nan_to_num(x.float(), nan=0.0, posinf=SATURATE, neginf=-SATURATE).clamp(-SATURATE, SATURATE))
     lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    scale, zero = ((hi - lo) / 15.0).half(), lo.half()
+    scale, zero = _over(hi - lo, 15.0).half(), lo.half()
     codes = torch.where(scale > 0, (g - zero.float()) / scale.float(), 0.0).round().clamp(0.0, 15.0)
     return codes.to(torch.uint8).reshape(x.shape), scale[..., 0], zero[..., 0]
 
@@ -270,7 +275,7 @@ def _summary(case, k):
     """(mid, half-range, sigma) of every whole block of k [..., tokens, D]."""
     b = k.reshape(*k.shape[:-2], k.shape[-2] // _block(case), _block(case), k.shape[-1])
     lo, hi = b.amin(-2), b.amax(-2)
-    sigma = torch.maximum(lo.abs(), hi.abs()).amax(-1, keepdim=True) / 127.0
+    sigma = _over(torch.maximum(lo.abs(), hi.abs()).amax(-1, keepdim=True), 127.0)
     inverse = torch.where(sigma > 0, 1.0 / sigma, 0.0)
     return (((hi + lo) * 0.5) * inverse).round(), (((hi - lo) * 0.5) * inverse).round(), sigma[..., 0]
 
@@ -286,7 +291,7 @@ def _pick(state):
     L, S, H, g = case["layers"], case["seqs"], case["hkv"], case["hq"] // case["hkv"]
     q = state["q"].float().reshape(L, S, H, g, case["head_dim"])
     q = torch.where(q.isfinite(), q, 0.0)
-    tau = q.abs().amax(-1, keepdim=True) / 127.0
+    tau = _over(q.abs().amax(-1, keepdim=True), 127.0)
     a = (q * torch.where(tau > 0, 1.0 / tau, 0.0)).round().clamp(-127.0, 127.0)
     whole = torch.matmul(a, mid.mT) + torch.matmul(a.abs(), half.mT)  # whole numbers below 2^24
     score = ((whole * sigma[..., None, :]) * tau).amax(-2)  # [L, S, H, blocks]
@@ -367,12 +372,12 @@ def _exact_values(case, x):
     d = x.double().unflatten(-1, (D // G, G))
     if case["bits"] == 8:
         lo, hi = d.amin(-1, keepdim=True), d.amax(-1, keepdim=True)
-        scale = ((hi - lo).to(x.dtype).float() / 255.0).clamp_min(1e-8)
+        scale = ((hi - lo).to(x.dtype).double() / 255.0).float().clamp_min(1e-8)
         code = ((d - lo).to(x.dtype).float() / scale).clamp(0, 255).floor().half()
         return ((code * scale.half()) + lo.half()).flatten(-2).double()
     d = torch.nan_to_num(d, nan=0.0).clamp(-SATURATE, SATURATE)
     lo = d.amin(-1, keepdim=True)
-    s, z = ((d.amax(-1, keepdim=True) - lo) / 15.0).half().double(), lo.half().double()
+    s, z = ((d.amax(-1, keepdim=True) - lo).float().double() / 15.0).float().half().double(), lo.half().double()
     code = torch.where(s > 0, (d - z) / torch.where(s > 0, s, 1.0), 0.0).round().clamp(0, 15)
     return (code * s + z).flatten(-2)
 
@@ -384,11 +389,11 @@ def _exact_pick(case, q, k, length):
     b = k[:, : whole * B].reshape(H, whole, B, D)
     lo, hi = b.amin(2), b.amax(2)
     lo, hi = lo.float(), hi.float()  # a block's bounds are kept in f32
-    sigma = torch.maximum(lo.abs(), hi.abs()).amax(-1) / 127.0
+    sigma = (torch.maximum(lo.abs(), hi.abs()).amax(-1).double() / 127.0).float()
     inv = torch.where(sigma > 0, 1.0 / sigma, 0.0)[..., None]
     mid, half = ((0.5 * (hi + lo)) * inv).round().double(), ((0.5 * (hi - lo)) * inv).round().double()
     q = torch.nan_to_num(q.float(), nan=0.0, posinf=0.0, neginf=0.0).reshape(H, -1, D)
-    tau = q.abs().amax(-1) / 127.0
+    tau = (q.abs().amax(-1).double() / 127.0).float()
     a = (q * torch.where(tau > 0, 1.0 / tau, 0.0)[..., None]).round().clamp(-127, 127).double()
     total = torch.einsum("hgd,hbd->hgb", a, mid) + torch.einsum("hgd,hbd->hgb", a.abs(), half)
     score = ((total.float() * sigma[:, None, :]) * tau[..., None]).amax(1)
