@@ -87,10 +87,18 @@ enum {
 };
 
 /* Storage format of a pool: int8 codes with fp16 scale/zero per group (the
- * reference's QuantizedKVCache), or raw bf16 K/V (the unquantized KVCache of
+ * reference's QuantizedKVCache), raw bf16 K/V (the unquantized KVCache of
  * Sources/KrillCache/KVCache.swift:94, kept for comparison; head_dim 64 or 128,
- * bf16 k/v/q, no quantized snapshots or cascade). */
-enum { KRILL_KV_INT8 = 0, KRILL_KV_BF16 = 1 };
+ * bf16 k/v/q, no quantized snapshots or cascade), or 4-bit codes (no reference
+ * counterpart). 4 bits, per group of group_size elements:
+ *   scale = f16(f32(max - min) / 15), zero = f16(min)
+ *   code  = clip(round-half-even((x - zero) / scale), 0, 15), in f32 (scale 0: 0)
+ *   value = code * scale + zero in f32
+ * Inputs beyond +-61440 saturate and NaN counts as 0, so a 4-bit cache never
+ * holds an infinity or NaN. Every call of this header takes 4-bit pools except
+ * the disk tier; snapshots hold one code (0..15) per byte. KRILL_QUANT_F32
+ * and KRILL_ATTN_TENSOR_CORE only; k/v of an append must be 16-byte aligned. */
+enum { KRILL_KV_INT8 = 0, KRILL_KV_BF16 = 1, KRILL_KV_INT4 = 2 };
 
 typedef struct krill_pool_s* krill_pool_t;
 typedef uint64_t krill_seq_t;               /* generation << 32 | slot */
@@ -122,7 +130,8 @@ typedef struct {
                              dequantized once. 0 -> 256; < 0 -> off. Applies
                              to full-history pools with a tensor-core
                              implementation and split_tokens = 0.           */
-  int32_t kv_format;      /* KRILL_KV_INT8 (default) or KRILL_KV_BF16           */
+  int32_t kv_format;      /* KRILL_KV_INT8 (default), KRILL_KV_BF16 or
+                             KRILL_KV_INT4                                       */
   int64_t num_blocks;     /* pool capacity in 256-token blocks                  */
   int32_t wait_timeout_us; /* bound of every device-side wait in this pool's
                              kernels (a stage copy, a stage release), in
@@ -132,6 +141,10 @@ typedef struct {
                              device error flag and the kernel runs to its end
                              instead of hanging; that launch's outputs are
                              then not valid.                                */
+  int32_t block_summaries; /* 1: keep a summary (2 * head_dim + 4 bytes) of every
+                             full block of krill_pool_select_tokens() tokens per
+                             layer and kv head, for krill_select_blocks. Int8 or
+                             4-bit full-history pools. 0: none.               */
 } krill_pool_cfg;
 
 /* ---- errors ------------------------------------------------------------- */
@@ -240,7 +253,7 @@ krill_status_t krill_append_quantize(krill_pool_t pool, int32_t n_seqs, const kr
  * and sum rounded to f32 and the result rounded to `dtype` before it is
  * quantized. rope_cos / rope_sin: device f32 tables [rope_rows][head_dim/2]
  * owned by the caller (angle(p, d) = p * base^(-2d/head_dim)); positions must
- * stay below rope_rows. V is appended unrotated. int8 pools only. */
+ * stay below rope_rows. V is appended unrotated. int8 and 4-bit pools. */
 krill_status_t krill_append_quantize_rope(krill_pool_t pool, int32_t n_seqs, const krill_seq_t* seqs,
                                           int32_t layer_begin, int32_t layer_count, int32_t n_new,
                                           const void* k_new, const void* v_new, int32_t dtype,
@@ -282,6 +295,41 @@ krill_status_t krill_prefill_attention(krill_pool_t pool, int32_t n_seqs, const 
                                        int32_t layer_begin, int32_t layer_count, int32_t n_query,
                                        const void* q, int32_t q_dtype, void* out, int32_t out_dtype,
                                        float scale, void* stream);
+
+/* ---- block-sparse decode (no reference counterpart) ------------------------
+ * A long cache is cut into blocks of krill_pool_select_tokens() tokens (64; 32
+ * for int8 at head_dim 256). A pool created with block_summaries keeps, per
+ * full block, layer and kv head, each K channel's mid and half-range as whole
+ * numbers in -127..127 of sigma = max|k| / 127; the calls that write K
+ * (append, decode step, restore) keep them up to date. For a query head,
+ * rounded to whole numbers a of tau = max|q| / 127 (non-finite elements count
+ * as 0), a block scores
+ *     f32((sum_d a_d mid_d + |a_d| half_d) * sigma * tau)
+ * - the sum exact, the products rounded one after the other - an upper
+ * estimate of its largest q.k; a kv head's score is the largest of its query
+ * heads'. */
+krill_status_t krill_pool_select_tokens(krill_pool_t pool, int32_t* tokens);
+/* Per (layer, sequence, kv head) the max_blocks blocks to attend: the first
+ * first_blocks (>= 0) and the last last_blocks (>= 1) of the sequence always
+ * (max_blocks >= their sum), the rest by the largest scores, the lowest index
+ * among equal ones; every block where the sequence has no more than
+ * max_blocks. q as in krill_decode_attention. selected (device):
+ * [layer_count][n_seqs][num_kv_heads][max_blocks] block indices (position /
+ * block tokens), ascending, -1 past the last. */
+krill_status_t krill_select_blocks(krill_pool_t pool, int32_t n_seqs, const krill_seq_t* seqs,
+                                   int32_t layer_begin, int32_t layer_count, const void* q,
+                                   int32_t q_dtype, int32_t max_blocks, int32_t first_blocks,
+                                   int32_t last_blocks, int32_t* selected, void* stream);
+/* Decode attention over the picked blocks alone: krill_select_blocks, then
+ * krill_decode_attention with the softmax over the tokens of those blocks.
+ * scale must be positive. selected: receives the picked blocks as above, or
+ * NULL (pool scratch is used). With max_blocks covering a sequence the result
+ * is krill_decode_attention's within the attention tolerance. */
+krill_status_t krill_sparse_decode_attention(krill_pool_t pool, int32_t n_seqs, const krill_seq_t* seqs,
+                                             int32_t layer_begin, int32_t layer_count, const void* q,
+                                             int32_t q_dtype, void* out, int32_t out_dtype, float scale,
+                                             int32_t max_blocks, int32_t first_blocks,
+                                             int32_t last_blocks, int32_t* selected, void* stream);
 
 /* Allocation-free decode attention. No counterpart in the reference: it
  * exists for callers that cannot have the library allocate memory while they
@@ -362,6 +410,16 @@ krill_status_t krill_seq_snapshot_quantized(krill_pool_t pool, krill_seq_t seq, 
  * reference's dequantize (:200-204). Output [Hkv][S][D] f16 each. */
 krill_status_t krill_seq_snapshot_dequantized(krill_pool_t pool, krill_seq_t seq, int32_t layer,
                                               void* keys, void* values, void* stream);
+/* Rows [starts[i], starts[i] + n_rows) of each sequence and layer, dequantized
+ * (no reference counterpart): what an append of those rows stored, in the
+ * append's layout, keys / values [layer_count][n_seqs][Hkv][n_rows][D] of
+ * dtype F16, BF16 or F32 (either may be NULL; 16-byte aligned), each value
+ * rounded once to it (int8 pools: the reference's two f16 roundings come
+ * first). starts: host array, or NULL for the first retained row of each
+ * sequence. int8 and 4-bit pools. */
+krill_status_t krill_read_rows(krill_pool_t pool, int32_t n_seqs, const krill_seq_t* seqs,
+                               int32_t layer_begin, int32_t layer_count, const int64_t* starts,
+                               int64_t n_rows, void* keys, void* values, int32_t dtype, void* stream);
 /* restoreQuantized(_:) for one layer (QuantizedKVCache.swift:122-129): copy
  * (never alias) `rows` rows in the snapshot layout into the sequence; the
  * layer's length becomes total_seen (= rows on a full-history pool; on a

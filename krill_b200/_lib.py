@@ -24,7 +24,7 @@ KRILL_ERR_NO_DEVICE = 7
 DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_U8 = 0, 1, 2, 3
 QUANT_F32, QUANT_INPUT_DTYPE = 0, 1
 ATTN_TENSOR_CORE, ATTN_CUDA_CORE, ATTN_TENSOR_CORE_SYNC, ATTN_TENSOR_CORE_PAIR = 0, 1, 2, 3
-KV_INT8, KV_BF16 = 0, 1
+KV_INT8, KV_BF16, KV_INT4 = 0, 1, 2
 DEVICE_ERR_TIMEOUT = 1
 
 _STATUS_NAMES = {
@@ -55,6 +55,7 @@ class PoolCfg(C.Structure):
         ("kv_format", C.c_int32),
         ("num_blocks", C.c_int64),
         ("wait_timeout_us", C.c_int32),
+        ("block_summaries", C.c_int32),
     ]
 
 
@@ -99,6 +100,11 @@ _SIGS = {
     "krill_append_quantize": (i32, [vp, i32, P_u64, i32, i32, i32, vp, vp, i32, vp]),
     "krill_verify_attention": (i32, [vp, i32, P_u64, i32, i32, i32, vp, i32, vp, i32, C.c_float, vp]),
     "krill_prefill_attention": (i32, [vp, i32, P_u64, i32, i32, i32, vp, i32, vp, i32, C.c_float, vp]),
+    "krill_pool_select_tokens": (i32, [vp, P_i32]),
+    "krill_select_blocks": (i32, [vp, i32, P_u64, i32, i32, vp, i32, i32, i32, i32, vp, vp]),
+    "krill_sparse_decode_attention": (i32, [vp, i32, P_u64, i32, i32, vp, i32, vp, i32, f32, i32, i32, i32,
+                                            vp, vp]),
+    "krill_read_rows": (i32, [vp, i32, P_u64, i32, i32, P_i64, i64, vp, vp, i32, vp]),
     "krill_append_quantize_rope": (i32, [vp, i32, P_u64, i32, i32, i32, vp, vp, i32, vp, vp, i64, vp]),
     "krill_decode_attention": (i32, [vp, i32, P_u64, i32, i32, vp, i32, vp, i32, f32, vp]),
     "krill_decode_attention_noalloc": (i32, [vp, i32, P_u64, i32, i32, vp, i32, vp, i32, f32, vp]),

@@ -58,17 +58,19 @@ def _seq_array(seqs: Sequence["Sequence_"]):
 
 class KVPool:
     """One device-resident block pool for a layer group (256-token blocks,
-    int8 codes + fp16 scale/zero per group). ``device=-1`` makes a host-only
-    pool (accounting and prefix logic only)."""
+    int8 or 4-bit codes + fp16 scale/zero per group, ``kv_format``).
+    ``block_summaries`` keeps what ``select_blocks`` and
+    ``sparse_decode_attention`` score blocks by. ``device=-1`` makes a
+    host-only pool (accounting and prefix logic only)."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, num_q_heads: int, head_dim: int,
                  num_blocks: int, group_size: int = 64, window: int = 0, max_append: int = 0,
                  quant_variant: int = L.QUANT_F32, attn_impl: int = L.ATTN_TENSOR_CORE,
                  split_tokens: int = 0, cascade_min_tokens: int = 0, kv_format: int = L.KV_INT8,
-                 device: int = 0, wait_timeout_us: int = 0):
+                 device: int = 0, wait_timeout_us: int = 0, block_summaries: bool = False):
         cfg = L.PoolCfg(num_layers, num_kv_heads, num_q_heads, head_dim, group_size, window,
                         max_append, quant_variant, attn_impl, split_tokens, cascade_min_tokens,
-                        kv_format, num_blocks, wait_timeout_us)
+                        kv_format, num_blocks, wait_timeout_us, int(block_summaries))
         h = C.c_void_p()
         check(L.lib.krill_pool_create(C.byref(cfg), device, C.byref(h)))
         self.handle = h
@@ -94,6 +96,13 @@ class KVPool:
     def block_bytes(self) -> int:
         v = C.c_int64()
         check(L.lib.krill_pool_block_bytes(self.handle, C.byref(v)))
+        return v.value
+
+    @property
+    def select_tokens(self) -> int:
+        """Tokens of a block that ``select_blocks`` picks."""
+        v = C.c_int32()
+        check(L.lib.krill_pool_select_tokens(self.handle, C.byref(v)))
         return v.value
 
     @property
@@ -372,6 +381,65 @@ def decode_attention(pool: KVPool, seqs, layer_begin: int, q, out, scale: float,
     check(L.lib.krill_decode_attention(pool.handle, ns, arr, layer_begin, lc, _ptr(q), _dt(q),
                                        _ptr(out), _dt(out), scale, _stream(stream)))
     return out
+
+
+def select_blocks(pool: KVPool, seqs, layer_begin: int, q, max_blocks: int, first_blocks: int = 1,
+                  last_blocks: int = 1, selected=None, stream=None):
+    """Blocks of ``pool.select_tokens`` tokens that each (layer, sequence, kv
+    head) should attend for the query q [layer_count, n_seqs, Hq, D]: int32
+    indices [layer_count, n_seqs, Hkv, max_blocks], ascending, -1 past the last
+    (krill_select_blocks)."""
+    lc, ns = q.shape[0], q.shape[1]
+    assert ns == len(seqs)
+    selected = _selected(pool, lc, ns, max_blocks, selected, q.device)
+    check(L.lib.krill_select_blocks(pool.handle, ns, _seq_array(seqs), layer_begin, lc, _ptr(q), _dt(q), max_blocks,
+                                    first_blocks, last_blocks, _ptr(selected), _stream(stream)))
+    return selected
+
+
+def sparse_decode_attention(pool: KVPool, seqs, layer_begin: int, q, out, scale: float, max_blocks: int,
+                            first_blocks: int = 1, last_blocks: int = 1, selected=None, return_blocks: bool = False,
+                            stream=None):
+    """decode_attention over the blocks that ``select_blocks`` picks. q/out:
+    [layer_count, n_seqs, Hq, D]. Returns out, or (out, picked blocks) with
+    ``return_blocks`` or a ``selected`` buffer."""
+    lc, ns = q.shape[0], q.shape[1]
+    assert ns == len(seqs)
+    if return_blocks or selected is not None:
+        selected = _selected(pool, lc, ns, max_blocks, selected, q.device)
+    check(L.lib.krill_sparse_decode_attention(pool.handle, ns, _seq_array(seqs), layer_begin, lc, _ptr(q), _dt(q),
+                                              _ptr(out), _dt(out), scale, max_blocks, first_blocks, last_blocks,
+                                              _ptr(selected), _stream(stream)))
+    return out if selected is None else (out, selected)
+
+
+def _selected(pool: KVPool, lc: int, ns: int, max_blocks: int, selected, device):
+    shape = (lc, ns, pool.num_kv_heads, max(0, max_blocks))
+    if selected is None:
+        return torch.empty(shape, dtype=torch.int32, device=device)
+    if tuple(selected.shape) != shape or selected.dtype != torch.int32:
+        raise ValueError(f"selected must be int32 {list(shape)}")
+    return selected
+
+
+def read_rows(pool: KVPool, seqs, layer_begin: int, layer_count: int, n_rows: int, starts=None, dtype=None,
+              keys=None, values=None, stream=None):
+    """Cached rows [starts[i], starts[i] + n_rows) of each sequence, dequantized:
+    (keys, values) [layer_count, n_seqs, Hkv, n_rows, D], f16 unless ``dtype``
+    (or given outputs) say otherwise. ``starts`` defaults to the first retained
+    row (krill_read_rows)."""
+    shape = (layer_count, len(seqs), pool.num_kv_heads, max(0, n_rows), pool.head_dim)
+    dtype = dtype or (keys.dtype if keys is not None else torch.float16)
+    dev = torch.device("cuda", pool.device)
+    keys = torch.empty(shape, dtype=dtype, device=dev) if keys is None else keys
+    values = torch.empty(shape, dtype=dtype, device=dev) if values is None else values
+    for t, name in ((keys, "keys"), (values, "values")):
+        if tuple(t.shape) != shape or t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype} {list(shape)}")
+    st = None if starts is None else (C.c_int64 * max(1, len(seqs)))(*starts)
+    check(L.lib.krill_read_rows(pool.handle, len(seqs), _seq_array(seqs), layer_begin, layer_count, st, n_rows,
+                                _ptr(keys), _ptr(values), _dt(keys), _stream(stream)))
+    return keys, values
 
 
 def decode_step(pool: KVPool, seqs, layer_begin: int, k_new, v_new, q, out, scale: float, stream=None):

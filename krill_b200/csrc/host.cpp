@@ -104,6 +104,7 @@ struct DeferredAppend {
   const void* k = nullptr;
   const void* v = nullptr;
   bool pending = false;  // planned, not launched yet
+  std::vector<SumItem> sums;  // sub-blocks that the append completes (pools with summaries)
 };
 
 // Decode-attention planner buffers, reused across calls.
@@ -155,6 +156,12 @@ struct krill_pool_s {
   float* d_partials = nullptr;
   int64_t partials_cap = 0;
   unsigned long long* d_split_ctr = nullptr;  // arrival counters, one per partial record
+  uint8_t* d_sel = nullptr;  // picked blocks of a sparse decode, then score keys of very long sequences
+  int64_t sel_cap = 0;
+  // the last attention call that used the pool's scratch: its stream, and the
+  // event of its staging slot, which marks the end of its kernels
+  cudaStream_t scratch_stream = nullptr;
+  cudaEvent_t scratch_ev = nullptr;
   uint32_t attn_epoch = 0;                    // launches of the decode kernel (never 0 in use)
   int64_t kernels = 0;  // device kernels launched since the last krill_pool_kernel_count
   std::map<std::string, uint8_t*> ipc_maps;  // other processes' pools opened here (handle bytes)
@@ -366,10 +373,40 @@ krill_status_t check_aligned(const void* ptr, const char* what) {
   return KRILL_OK;
 }
 
+// Scratch of the pool is about to be used on `stream`: a call on another
+// stream that used it last is waited for (on the device).
+krill_status_t scratch_acquire(krill_pool_t p, cudaStream_t stream) {
+  if (p->scratch_ev && p->scratch_stream != stream) CUDA_TRY(cudaStreamWaitEvent(stream, p->scratch_ev, 0));
+  return KRILL_OK;
+}
+
 krill_status_t check_layers(krill_pool_t p, int32_t lb, int32_t lc) {
   if (lb < 0 || lc < 0 || lb + lc > p->geom.L)
     return fail(KRILL_ERR_INVALID, "layer range [%d, %d) outside [0, %d)", lb, lb + lc, p->geom.L);
   return KRILL_OK;
+}
+
+// Appends the full sub-blocks [first, last) of one layer to `out`, for their
+// summaries.
+void add_summaries(krill_pool_t p, const Seq& s, int layer, int64_t first, int64_t last, std::vector<SumItem>* out) {
+  for (int64_t sb = first; sb < last; ++sb)
+    out->push_back(SumItem{s.blocks[(size_t)(sb / p->geom.spb)], layer, (int32_t)(sb % p->geom.spb)});
+}
+
+// Uploads and launches the summaries of `sums` (their K/V are in place on `stream`).
+krill_status_t run_summaries(krill_pool_t p, const std::vector<SumItem>& sums, cudaStream_t stream) {
+  if (sums.empty()) return KRILL_OK;
+  StageSlot* slot = nullptr;
+  const size_t bytes = sums.size() * sizeof(SumItem);
+  TRY(stage_acquire(p, bytes, &slot));
+  std::memcpy(slot->h, sums.data(), bytes);
+  TRY(stage_upload(slot, bytes, stream));
+  CUDA_TRY(timed_launch(p, 1, stream, [&] {
+    return launch_summaries(p->geom, p->d_pool, reinterpret_cast<const SumItem*>(slot->d), (int64_t)sums.size(),
+                            stream);
+  }));
+  p->kernels += 1;
+  return stage_release(slot, stream);
 }
 
 // ---------------------------------------------------------------- append
@@ -388,7 +425,7 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
   TRY(check_layers(p, lb, lc));
   TRY(check_dtype16(dtype, "k/v"));
   if (rope.cos) {
-    if (p->geom.fmt != kFmtInt8) return fail(KRILL_ERR_INVALID, "the RoPE append needs an int8 pool");
+    if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "the RoPE append needs an int8 or 4-bit pool");
     if (!rope.sin) return fail(KRILL_ERR_INVALID, "null rope_sin");
     if ((reinterpret_cast<uintptr_t>(rope.cos) | reinterpret_cast<uintptr_t>(rope.sin)) & 3)
       return fail(KRILL_ERR_INVALID, "rope tables must be 4-byte aligned");
@@ -398,6 +435,10 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
   if (n_seqs < 0 || n_new < 0) return fail(KRILL_ERR_INVALID, "negative count");
   if (n_seqs == 0 || lc == 0 || n_new == 0) return KRILL_OK;
   if (!seqs || (!p->host_only && (!k || !v))) return fail(KRILL_ERR_INVALID, "null k/v/seqs");
+  if (p->geom.fmt == kFmtInt4) {
+    TRY(check_aligned(k, "k"));
+    TRY(check_aligned(v, "v"));
+  }
   if (p->windowed() && n_new > p->cfg.max_append)
     return fail(KRILL_ERR_INVALID, "n_new %d exceeds the windowed pool's max_append %d", n_new,
                 p->cfg.max_append);
@@ -412,8 +453,8 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
         if (sv[i]->len[lb + li] + n_new > rope.rows)
           return fail(KRILL_ERR_INVALID, "position %lld beyond the %lld-row rope table",
                       (long long)(sv[i]->len[lb + li] + n_new - 1), (long long)rope.rows);
-  // tiled appends (int8 pools) take one entry per touched sub-block
-  const bool tiled = append_uses_tiles(n_new) && p->geom.fmt == kFmtInt8;
+  // tiled appends (quantized pools) take one entry per touched sub-block
+  const bool tiled = append_uses_tiles(n_new) && p->geom.fmt != kFmtBf16;
   const int n_chunks = append_tile_chunks(n_new, p->geom.subt);
   const size_t n_dst = (size_t)lc * n_seqs * (tiled ? n_chunks : n_new);
   StageSlot* slot = nullptr;
@@ -426,7 +467,9 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
     dry.resize(n_dst);
     dst = dry.data();
   } else {
-    TRY(stage_acquire(p, n_dst * sizeof(AppendDst), &slot));
+    // the sub-blocks whose summaries the call completes follow the destinations
+    const size_t n_sums = p->geom.sum_off ? (size_t)lc * n_seqs * (size_t)(n_new / p->geom.subt + 1) : 0;
+    TRY(stage_acquire(p, align16(n_dst * sizeof(AppendDst)) + n_sums * sizeof(SumItem), &slot));
     dst = reinterpret_cast<AppendDst*>(slot->h);
   }
   for (int si = 0; si < n_seqs; ++si) {
@@ -459,7 +502,15 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
       }
     }
   }
+  std::vector<SumItem> sums;
+  if (p->geom.sum_off && !p->host_only)
+    for (int si = 0; si < n_seqs; ++si)
+      for (int li = 0; li < lc; ++li) {
+        const int64_t len = sv[si]->len[lb + li];
+        add_summaries(p, *sv[si], lb + li, len / p->geom.subt, (len + n_new) / p->geom.subt, &sums);
+      }
   if (deferred && !p->host_only) {
+    deferred->sums = std::move(sums);
     deferred->lb = lb;
     deferred->lc = lc;
     deferred->n_seqs = n_seqs;
@@ -469,12 +520,18 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
     deferred->v = v;
     deferred->pending = true;
   } else if (!p->host_only) {
-    TRY(stage_upload(slot, n_dst * sizeof(AppendDst), stream));
+    const size_t dst_bytes = n_dst * sizeof(AppendDst), sum_at = align16(dst_bytes);
+    if (!sums.empty()) std::memcpy(slot->h + sum_at, sums.data(), sums.size() * sizeof(SumItem));
+    TRY(stage_upload(slot, sums.empty() ? dst_bytes : sum_at + sums.size() * sizeof(SumItem), stream));
     CUDA_TRY(timed_launch(p, 1, stream, [&] {
-      return launch_append(p->geom, p->d_pool, reinterpret_cast<const AppendDst*>(slot->d), lb, lc,
-                           n_seqs, n_new, k, v, dtype, p->d_err + 1, rope, stream);
+      const cudaError_t e =
+          launch_append(p->geom, p->d_pool, reinterpret_cast<const AppendDst*>(slot->d), lb, lc, n_seqs, n_new, k, v,
+                        dtype, p->d_err + 1, rope, stream);
+      if (e != cudaSuccess || sums.empty()) return e;
+      return launch_summaries(p->geom, p->d_pool, reinterpret_cast<const SumItem*>(slot->d + sum_at),
+                              (int64_t)sums.size(), stream);
     }));
-    p->kernels += 1;
+    p->kernels += 1 + (sums.empty() ? 0 : 1);
     TRY(stage_release(slot, stream));
   }
   for (int si = 0; si < n_seqs; ++si) {
@@ -517,6 +574,15 @@ krill_status_t flush_deferred_append(krill_pool_t p, DeferredAppend& da, cudaStr
   return stage_release(slot, stream);
 }
 
+// The summaries of the sub-blocks that a deferred append completed, after the
+// attention of its step (which does not read them).
+krill_status_t run_deferred_summaries(krill_pool_t p, DeferredAppend& da, cudaStream_t stream) {
+  if (da.pending || da.sums.empty()) return KRILL_OK;
+  const krill_status_t st = run_summaries(p, da.sums, stream);
+  da.sums.clear();
+  return st;
+}
+
 // ---------------------------------------------------------------- attention
 krill_status_t ensure_scratch(krill_pool_t p, int64_t records, int64_t /*unused*/) {
   const int64_t pf = partial_floats(p->geom.D);
@@ -538,17 +604,81 @@ krill_status_t ensure_scratch(krill_pool_t p, int64_t records, int64_t /*unused*
   return KRILL_OK;
 }
 
+// Block choice of a sparse decode: budget blocks per (layer, sequence, kv
+// head), the first / last ones among them always; out: the caller's index
+// buffer, or nullptr.
+struct SelectSpec {
+  int32_t budget, first, last;
+  int32_t* out;
+};
+
+krill_status_t check_select(krill_pool_t p, const SelectSpec& sp) {
+  if (!p->geom.sum_off)
+    return fail(KRILL_ERR_INVALID, "block choice needs a pool with block summaries (krill_pool_cfg.block_summaries)");
+  if (sp.first < 0 || sp.last < 1)
+    return fail(KRILL_ERR_INVALID, "first_blocks must be >= 0 and last_blocks >= 1");
+  if (sp.budget < 1 || (int64_t)sp.budget < (int64_t)sp.first + sp.last)
+    return fail(KRILL_ERR_INVALID, "max_blocks %d is below first_blocks + last_blocks", sp.budget);
+  return KRILL_OK;
+}
+
+// Scratch for the picked blocks (when the caller gives no buffer) and for the
+// keys of sequences whose blocks do not fit shared memory. Fills sp->sel,
+// scratch and scratch_stride.
+krill_status_t ensure_select(krill_pool_t p, const SelectSpec& spec, int64_t pairs, int64_t max_n, SelectParams* sp) {
+  const int64_t sel_bytes = spec.out ? 0 : (int64_t)align16((size_t)pairs * spec.budget * 4);
+  const int64_t key_bytes = max_n > kSelectSmemKeys ? pairs * max_n * 4 : 0;
+  if (sel_bytes + key_bytes > p->sel_cap) {
+    CUDA_TRY(cudaDeviceSynchronize());  // kernels in flight may still use the old buffer
+    if (p->d_sel) cudaFree(p->d_sel);
+    p->d_sel = nullptr;
+    p->sel_cap = 0;
+    const int64_t cap = std::max<int64_t>((sel_bytes + key_bytes) * 3 / 2, 1 << 20);
+    if (cudaMalloc(&p->d_sel, (size_t)cap) != cudaSuccess) {
+      p->d_sel = nullptr;
+      cudaGetLastError();
+      return fail(KRILL_ERR_OOM, "no memory for %lld bytes of picked blocks", (long long)cap);
+    }
+    p->sel_cap = cap;
+  }
+  sp->sel = spec.out ? spec.out : reinterpret_cast<int32_t*>(p->d_sel);
+  sp->scratch = key_bytes ? reinterpret_cast<uint32_t*>(p->d_sel + sel_bytes) : nullptr;
+  sp->scratch_stride = max_n;
+  return KRILL_OK;
+}
+
+SelectParams select_params(krill_pool_t p, const SelectSpec& spec, const void* q, int32_t q_dtype) {
+  const Geom& g = p->geom;
+  SelectParams sp{};
+  sp.pool = p->d_pool;
+  sp.page_bytes = g.page_bytes;
+  sp.sum_off = g.sum_off;
+  sp.L = g.L;
+  sp.Hkv = g.Hkv;
+  sp.Hq = g.Hq;
+  sp.g = g.g;
+  sp.spb = g.spb;
+  sp.T = g.subt;
+  sp.q = q;
+  sp.q_dtype = q_dtype;
+  sp.budget = spec.budget;
+  sp.first = spec.first;
+  sp.last = spec.last;
+  return sp;
+}
+
 krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs, int32_t lb,
                             int32_t lc, const void* q, int32_t q_dtype, void* out,
                             int32_t out_dtype, float scale, cudaStream_t stream,
-                            int32_t n_query = 1, DeferredAppend* pre = nullptr) {
+                            int32_t n_query = 1, DeferredAppend* pre = nullptr,
+                            const SelectSpec* sel = nullptr) {
   TRY(check_layers(p, lb, lc));
   if (n_query < 1) return fail(KRILL_ERR_INVALID, "n_query must be positive");
   if (n_query > 1 && p->windowed())
     return fail(KRILL_ERR_INVALID, "multi-query verify attention needs a full-history pool");
   // Many queries per sequence (chunked prefill, long verify) run as causal
   // tcgen05 cascade items: the sequence's K/V is read once per query block.
-  const bool causal_path = n_query > 1 && p->geom.fmt == kFmtInt8 &&
+  const bool causal_path = n_query > 1 && p->geom.fmt != kFmtBf16 &&
                            shared_uses_umma(p->geom, p->cfg.attn_impl) &&
                            (int64_t)n_query * p->geom.g >= 64;
   TRY(check_dtype16(q_dtype, "q"));
@@ -581,7 +711,8 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   pl.gshared.clear();
   pl.seq_sh.assign((size_t)n_seqs, 0);
   const int64_t min_tok = p->cfg.cascade_min_tokens == 0 ? 256 : p->cfg.cascade_min_tokens;
-  if (!p->windowed() && g.fmt == kFmtInt8 && p->cfg.attn_impl != KRILL_ATTN_CUDA_CORE &&
+  if (!p->windowed() && !sel && p->cfg.attn_impl != KRILL_ATTN_CUDA_CORE &&
+      (g.fmt == kFmtInt8 || (g.fmt == kFmtInt4 && shared_uses_umma(g, p->cfg.attn_impl))) &&
       p->cfg.split_tokens == 0 && n_query == 1 &&
       p->cfg.cascade_min_tokens >= 0 && n_seqs >= 2) {
     const size_t min_blocks = (size_t)std::max<int64_t>(1, (min_tok + kBlockTokens - 1) / kBlockTokens);
@@ -640,7 +771,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   // tile, each column masked at its own query's bound (AttnUnit::nq), so the
   // cache is read once per unit instead of once per query; otherwise (and on
   // the causal cascade path) one unit per query.
-  const int fold = (n_query > 1 && !causal_path && g.fmt == kFmtInt8 &&
+  const int fold = (n_query > 1 && !causal_path && g.fmt != kFmtBf16 &&
                     p->cfg.attn_impl != KRILL_ATTN_CUDA_CORE)
                        ? std::max(1, std::min(n_query, 8 / g.g))
                        : 1;
@@ -650,12 +781,12 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   // the first one's items, so each sub-block is staged once for both; the
   // shadow keeps its own queries, bounds and partial records, and has no
   // items of its own.
-  const bool qt2 = q_units == 2 && !causal_path && g.fmt == kFmtInt8 && g.D <= 128 &&
+  const bool qt2 = q_units == 2 && !causal_path && g.fmt != kFmtBf16 && g.D <= 128 &&
                    g.Hkv >= 8 && p->cfg.attn_impl != KRILL_ATTN_CUDA_CORE;
   const int64_t n_units = (int64_t)lc * n_seqs * q_units;
   pl.units.resize((size_t)n_units);
   pl.nsb.resize((size_t)n_units);
-  int64_t total_sb = 0;
+  int64_t total_sb = 0, max_n = 0;
   for (int li = 0; li < lc; ++li) {
     const int L = lb + li;
     for (int si = 0; si < n_seqs; ++si) {
@@ -681,6 +812,10 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
         pl.nsb[ui] = causal_path ? 0
                                  : (t_hi + g.subt - 1) / g.subt -
                                        std::max<int64_t>(t_lo / g.subt, pl.seq_sh[si]);
+        if (sel) {  // the unit's items index its picked blocks
+          max_n = std::max(max_n, pl.nsb[ui]);
+          pl.nsb[ui] = std::min<int64_t>(pl.nsb[ui], sel->budget);
+        }
         total_sb += pl.nsb[ui];
         if (qt2 && k == 1) {  // the shadow's range is the pair's: its items cover both
           total_sb -= pl.nsb[ui - 1];
@@ -794,7 +929,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   // half of every sub-block); a pair then takes the place of one CTA in the
   // split below.
   bool sh_pair = false;
-  if (!pl.pairs.empty() && p->cfg.attn_impl == KRILL_ATTN_TENSOR_CORE_PAIR && p->pair_slots > 0 &&
+  if (!pl.pairs.empty() && g.fmt == kFmtInt8 && p->cfg.attn_impl == KRILL_ATTN_TENSOR_CORE_PAIR && p->pair_slots > 0 &&
       shared_uses_umma(g, p->cfg.attn_impl))
     for (const Plan::Pair& pr : pl.pairs) sh_pair = sh_pair || pr.n_rows > 128;
   if (!pl.pairs.empty()) {
@@ -913,7 +1048,12 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     }
     pl.items.swap(pl.items_tmp);
   }
-  if (!p->host_only) TRY(ensure_scratch(p, split_count * g.Hkv, 0));
+  SelectParams selp{};
+  if (sel) selp = select_params(p, *sel, q, q_dtype);
+  if (!p->host_only) {
+    TRY(ensure_scratch(p, split_count * g.Hkv, 0));
+    if (sel) TRY(ensure_select(p, *sel, n_units * g.Hkv, max_n, &selp));
+  }
   // ---- longest-processing-time assignment of items to persistent CTAs ----
   // Items are at most C sub-blocks, so a counting sort orders them by size.
   const int64_t n_items = (int64_t)pl.items.size();
@@ -1029,9 +1169,13 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     dp.split_ctr = merge_in_kernel ? &ctr_tag : nullptr;
     dp.sh_grid = sh_grid;
     dp.sh_pair = sh_pair ? 1 : 0;
+    static const int32_t sel_tag = 0;
+    dp.sel = sel ? &sel_tag : nullptr;
     describe_attention(g, dp, grid, p->cfg.attn_impl, pl.last_kernels, sizeof(pl.last_kernels));
   }
   if (p->host_only) return KRILL_OK;  // dry run: planned, nothing launched
+  const bool uses_scratch = split_count > 0 || sel;
+  if (uses_scratch) TRY(scratch_acquire(p, stream));
   TRY(stage_upload(slot, total, stream));
   AttnParams ap{};
   ap.pool = p->d_pool;
@@ -1082,10 +1226,84 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     // between them): let it start while the append runs
     ap.pdl = (sh_grid == 0 && grid > 0 && p->cfg.attn_impl != KRILL_ATTN_CUDA_CORE) ? 1 : 0;
   }
+  if (sel) {
+    selp.units = ap.units;
+    selp.bt = ap.bt;
+    selp.bt_stride = ap.bt_stride;
+    CUDA_TRY(timed_launch(p, 0, stream, [&] { return launch_select(g, selp, (int)n_units, max_n, p->num_sms, stream); }));
+    p->kernels += 1;
+    ap.sel = selp.sel;
+    ap.sel_stride = sel->budget;
+    ap.pdl = 1;  // the decode kernel starts up while the choice runs
+  }
   CUDA_TRY(timed_launch(p, 0, stream, [&] { return launch_attention(g, ap, grid, p->cfg.attn_impl, stream); }));
   p->kernels += (grid > 0 ? 1 : 0) + (attn_needs_combine(ap, grid, p->cfg.attn_impl) ? 1 : 0) +
                 (sh_grid > 0 ? 1 : 0);
   TRY(stage_release(slot, stream));
+  if (uses_scratch) {
+    p->scratch_stream = stream;
+    p->scratch_ev = slot->ev;
+  }
+  return KRILL_OK;
+}
+
+// The block choice alone: picked indices into spec.out.
+krill_status_t do_select(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs, int32_t lb, int32_t lc,
+                         const void* q, int32_t q_dtype, const SelectSpec& spec, cudaStream_t stream) {
+  TRY(check_layers(p, lb, lc));
+  TRY(check_dtype16(q_dtype, "q"));
+  TRY(check_select(p, spec));
+  if (n_seqs < 0) return fail(KRILL_ERR_INVALID, "negative n_seqs");
+  if (n_seqs == 0 || lc == 0) return KRILL_OK;
+  if (!seqs || (!p->host_only && (!q || !spec.out))) return fail(KRILL_ERR_INVALID, "null q/selected/seqs");
+  TRY(check_aligned(q, "q"));
+  if ((uintptr_t)spec.out & 3) return fail(KRILL_ERR_INVALID, "selected must be 4-byte aligned");
+  const Geom& g = p->geom;
+  Plan& pl = p->plan;
+  pl.sv.resize(n_seqs);
+  int64_t bt_stride = 1, max_n = 1;
+  for (int i = 0; i < n_seqs; ++i) {
+    TRY(seq_get(p, seqs[i], &pl.sv[i]));
+    bt_stride = std::max<int64_t>(bt_stride, (int64_t)pl.sv[i]->blocks.size());
+  }
+  const int64_t n_units = (int64_t)lc * n_seqs;
+  pl.units.assign((size_t)n_units, AttnUnit{});
+  for (int li = 0; li < lc; ++li)
+    for (int si = 0; si < n_seqs; ++si) {
+      const int64_t len = pl.sv[si]->len[lb + li];
+      if (len <= 0) return fail(KRILL_ERR_INVALID, "block choice over an empty cache (layer %d)", lb + li);
+      AttnUnit& u = pl.units[(size_t)li * n_seqs + si];
+      u.qo_row = li * n_seqs + si;
+      u.si = si;
+      u.layer = lb + li;
+      u.t_hi = (int32_t)len;
+      max_n = std::max<int64_t>(max_n, (len + g.subt - 1) / g.subt);
+    }
+  if (p->host_only) return KRILL_OK;
+  SelectParams sp = select_params(p, spec, q, q_dtype);
+  TRY(ensure_select(p, spec, n_units * g.Hkv, max_n, &sp));
+  const size_t units_bytes = align16((size_t)n_units * sizeof(AttnUnit));
+  const size_t bt_bytes = (size_t)n_seqs * bt_stride * sizeof(int32_t);
+  StageSlot* slot = nullptr;
+  TRY(stage_acquire(p, units_bytes + bt_bytes, &slot));
+  std::memcpy(slot->h, pl.units.data(), (size_t)n_units * sizeof(AttnUnit));
+  int32_t* bt = reinterpret_cast<int32_t*>(slot->h + units_bytes);
+  for (int si = 0; si < n_seqs; ++si) {
+    const auto& blocks = pl.sv[si]->blocks;
+    for (int64_t j = 0; j < bt_stride; ++j) bt[si * bt_stride + j] = j < (int64_t)blocks.size() ? blocks[j] : -1;
+  }
+  if (sp.scratch) TRY(scratch_acquire(p, stream));
+  TRY(stage_upload(slot, units_bytes + bt_bytes, stream));
+  sp.units = reinterpret_cast<const AttnUnit*>(slot->d);
+  sp.bt = reinterpret_cast<const int32_t*>(slot->d + units_bytes);
+  sp.bt_stride = (int)bt_stride;
+  CUDA_TRY(timed_launch(p, 0, stream, [&] { return launch_select(g, sp, (int)n_units, max_n, p->num_sms, stream); }));
+  p->kernels += 1;
+  TRY(stage_release(slot, stream));
+  if (sp.scratch) {
+    p->scratch_stream = stream;
+    p->scratch_ev = slot->ev;
+  }
   return KRILL_OK;
 }
 
@@ -1136,6 +1354,11 @@ krill_status_t do_restore(krill_pool_t p, Seq& s, int32_t layer, int64_t rows, i
                               p0, rows, in, p->d_err + 1, stream));
       p->kernels += 1;
       TRY(stage_release(slot, stream));
+      if (p->geom.sum_off) {
+        std::vector<SumItem> sums;
+        add_summaries(p, s, layer, 0, rows / p->geom.subt, &sums);
+        TRY(run_summaries(p, sums, stream));
+      }
     }
   }
   s.len[layer] = total_seen;
@@ -1186,8 +1409,22 @@ krill_status_t krill_pool_create(const krill_pool_cfg* cfg_in, int32_t device, k
   if (cfg.num_blocks <= 0 || cfg.num_blocks > INT32_MAX)
     return fail(KRILL_ERR_INVALID, "num_blocks out of range");
   if (cfg.wait_timeout_us < 0) return fail(KRILL_ERR_INVALID, "wait_timeout_us must be >= 0");
-  if (cfg.kv_format != KRILL_KV_INT8 && cfg.kv_format != KRILL_KV_BF16)
-    return fail(KRILL_ERR_INVALID, "kv_format must be KRILL_KV_INT8 or KRILL_KV_BF16");
+  if (cfg.kv_format != KRILL_KV_INT8 && cfg.kv_format != KRILL_KV_BF16 && cfg.kv_format != KRILL_KV_INT4)
+    return fail(KRILL_ERR_INVALID, "kv_format must be KRILL_KV_INT8, KRILL_KV_BF16 or KRILL_KV_INT4");
+  if (cfg.kv_format == KRILL_KV_INT4) {
+    if (cfg.attn_impl != KRILL_ATTN_TENSOR_CORE)
+      return fail(KRILL_ERR_INVALID, "4-bit pools use KRILL_ATTN_TENSOR_CORE");
+    if (cfg.quant_variant != KRILL_QUANT_F32)
+      return fail(KRILL_ERR_INVALID, "4-bit pools use KRILL_QUANT_F32");
+  }
+  if (cfg.block_summaries != 0 && cfg.block_summaries != 1)
+    return fail(KRILL_ERR_INVALID, "block_summaries must be 0 or 1");
+  if (cfg.block_summaries) {
+    if (cfg.window > 0) return fail(KRILL_ERR_INVALID, "block_summaries need a full-history pool (window 0)");
+    if (cfg.kv_format == KRILL_KV_BF16) return fail(KRILL_ERR_INVALID, "block_summaries need an int8 or 4-bit pool");
+    if (cfg.attn_impl == KRILL_ATTN_CUDA_CORE)
+      return fail(KRILL_ERR_INVALID, "block_summaries need a tensor-core attention");
+  }
   if (cfg.kv_format == KRILL_KV_BF16) {
     if (cfg.head_dim > 128) return fail(KRILL_ERR_INVALID, "bf16 pools support head_dim 64 and 128");
     if (cfg.attn_impl == KRILL_ATTN_CUDA_CORE)
@@ -1203,7 +1440,10 @@ krill_status_t krill_pool_create(const krill_pool_cfg* cfg_in, int32_t device, k
   p->cfg = cfg;
   p->geom = make_geom(cfg.num_layers, cfg.num_kv_heads, cfg.num_q_heads, cfg.head_dim,
                       cfg.group_size, ring, cfg.window, cfg.quant_variant,
-                      cfg.kv_format == KRILL_KV_BF16 ? kFmtBf16 : kFmtInt8);
+                      cfg.kv_format == KRILL_KV_BF16   ? kFmtBf16
+                      : cfg.kv_format == KRILL_KV_INT4 ? kFmtInt4
+                                                       : kFmtInt8,
+                      cfg.block_summaries != 0);
   p->device = device;
   p->host_only = device < 0;
   p->refcnt.assign((size_t)cfg.num_blocks, 0);
@@ -1275,6 +1515,7 @@ krill_status_t krill_pool_destroy(krill_pool_t p) {
     if (p->d_pool) cudaFree(p->d_pool);
     if (p->d_partials) cudaFree(p->d_partials);
     if (p->d_split_ctr) cudaFree(p->d_split_ctr);
+    if (p->d_sel) cudaFree(p->d_sel);
     if (p->d_err) cudaFree(p->d_err);
   }
   delete p;
@@ -1453,7 +1694,8 @@ krill_status_t krill_seq_memory_bytes(krill_pool_t p, krill_seq_t h, int32_t lay
   layer_span(p, *s, layer, &p0, &S);
   const Geom& g = p->geom;
   // QuantizedKVCache.memorySizeBytes: u8 K+V plus 4 f16 arrays per row (per group)
-  *bytes = 2 * S * g.Hkv * g.D + 4 * S * g.Hkv * g.NG * 2;
+  // (4-bit pools: half a byte per code)
+  *bytes = (g.fmt == kFmtInt4 ? 1 : 2) * S * g.Hkv * g.D + 4 * S * g.Hkv * g.NG * 2;
   return KRILL_OK;
 }
 
@@ -1550,6 +1792,90 @@ krill_status_t krill_verify_attention(krill_pool_t p, int32_t n_seqs, const kril
                       (cudaStream_t)stream, n_query);
 }
 
+krill_status_t krill_pool_select_tokens(krill_pool_t p, int32_t* tokens) {
+  if (!p || !tokens) return fail(KRILL_ERR_INVALID, "null argument");
+  *tokens = p->geom.subt;
+  return KRILL_OK;
+}
+
+krill_status_t krill_select_blocks(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs, int32_t layer_begin,
+                                   int32_t layer_count, const void* q, int32_t q_dtype, int32_t max_blocks,
+                                   int32_t first_blocks, int32_t last_blocks, int32_t* selected, void* stream) {
+  if (!p) return fail(KRILL_ERR_INVALID, "null pool");
+  std::lock_guard<std::recursive_mutex> lk(p->mu);
+  DeviceGuard dg(p->device);
+  return do_select(p, n_seqs, seqs, layer_begin, layer_count, q, q_dtype,
+                   SelectSpec{max_blocks, first_blocks, last_blocks, selected}, (cudaStream_t)stream);
+}
+
+krill_status_t krill_sparse_decode_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs,
+                                             int32_t layer_begin, int32_t layer_count, const void* q,
+                                             int32_t q_dtype, void* out, int32_t out_dtype, float scale,
+                                             int32_t max_blocks, int32_t first_blocks, int32_t last_blocks,
+                                             int32_t* selected, void* stream) {
+  if (!p) return fail(KRILL_ERR_INVALID, "null pool");
+  std::lock_guard<std::recursive_mutex> lk(p->mu);
+  DeviceGuard dg(p->device);
+  const SelectSpec spec{max_blocks, first_blocks, last_blocks, selected};
+  TRY(check_select(p, spec));
+  if (!(scale > 0.f)) return fail(KRILL_ERR_INVALID, "sparse decode needs a positive softmax scale");
+  if ((uintptr_t)selected & 3) return fail(KRILL_ERR_INVALID, "selected must be 4-byte aligned");
+  return do_attention(p, n_seqs, seqs, layer_begin, layer_count, q, q_dtype, out, out_dtype, scale,
+                      (cudaStream_t)stream, 1, nullptr, &spec);
+}
+
+krill_status_t krill_read_rows(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs, int32_t layer_begin,
+                               int32_t layer_count, const int64_t* starts, int64_t n_rows, void* keys, void* values,
+                               int32_t dtype, void* stream) {
+  if (!p) return fail(KRILL_ERR_INVALID, "null pool");
+  std::lock_guard<std::recursive_mutex> lk(p->mu);
+  DeviceGuard dg(p->device);
+  TRY(check_layers(p, layer_begin, layer_count));
+  if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "reading rows back needs an int8 or 4-bit pool");
+  if (dtype != KRILL_DTYPE_F16 && dtype != KRILL_DTYPE_BF16 && dtype != KRILL_DTYPE_F32)
+    return fail(KRILL_ERR_INVALID, "row dtype must be F16, BF16 or F32");
+  if (n_seqs < 0 || n_rows < 0) return fail(KRILL_ERR_INVALID, "negative count");
+  if (n_seqs == 0 || layer_count == 0 || n_rows == 0) return KRILL_OK;
+  if (!seqs) return fail(KRILL_ERR_INVALID, "null seqs");
+  TRY(check_aligned(keys, "keys"));
+  TRY(check_aligned(values, "values"));
+  Plan& pl = p->plan;
+  pl.sv.resize(n_seqs);
+  int64_t bt_stride = 1;
+  for (int i = 0; i < n_seqs; ++i) {
+    TRY(seq_get(p, seqs[i], &pl.sv[i]));
+    bt_stride = std::max<int64_t>(bt_stride, (int64_t)pl.sv[i]->blocks.size());
+    for (int L = layer_begin; L < layer_begin + layer_count; ++L) {
+      int64_t p0, S;
+      layer_span(p, *pl.sv[i], L, &p0, &S);
+      const int64_t start = starts ? starts[i] : p0;
+      if (start < p0 || n_rows > p0 + S - start)
+        return fail(KRILL_ERR_INVALID, "rows [%lld, %lld) of sequence %d are not cached (layer %d holds [%lld, %lld))",
+                    (long long)start, (long long)(start + n_rows), i, L, (long long)p0, (long long)(p0 + S));
+    }
+  }
+  TRY(require_device(p));
+  const size_t st_bytes = align16((size_t)n_seqs * sizeof(int64_t));
+  const size_t bt_bytes = (size_t)n_seqs * bt_stride * sizeof(int32_t);
+  StageSlot* slot = nullptr;
+  TRY(stage_acquire(p, st_bytes + bt_bytes, &slot));
+  int64_t* st = reinterpret_cast<int64_t*>(slot->h);
+  int32_t* bt = reinterpret_cast<int32_t*>(slot->h + st_bytes);
+  for (int i = 0; i < n_seqs; ++i) {
+    int64_t p0, S;
+    layer_span(p, *pl.sv[i], layer_begin, &p0, &S);
+    st[i] = starts ? starts[i] : p0;
+    const auto& blocks = pl.sv[i]->blocks;
+    for (int64_t j = 0; j < bt_stride; ++j) bt[i * bt_stride + j] = j < (int64_t)blocks.size() ? blocks[j] : -1;
+  }
+  TRY(stage_upload(slot, st_bytes + bt_bytes, (cudaStream_t)stream));
+  CUDA_TRY(launch_read_rows(p->geom, p->d_pool, reinterpret_cast<const int32_t*>(slot->d + st_bytes), (int)bt_stride,
+                            reinterpret_cast<const int64_t*>(slot->d), layer_begin, layer_count, n_seqs, n_rows, keys,
+                            values, dtype, (cudaStream_t)stream));
+  p->kernels += 1;
+  return stage_release(slot, (cudaStream_t)stream);
+}
+
 krill_status_t krill_prefill_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs,
                                        int32_t layer_begin, int32_t layer_count, int32_t n_query,
                                        const void* q, int32_t q_dtype, void* out, int32_t out_dtype,
@@ -1570,6 +1896,7 @@ krill_status_t krill_decode_step(krill_pool_t p, int32_t n_seqs, const krill_seq
   // upload per step, then the append and attention launches.
   DeferredAppend& da = p->deferred;
   da.pending = false;
+  da.sums.clear();
   TRY(do_append(p, n_seqs, seqs, layer_begin, layer_count, 1, k_new, v_new, kv_dtype,
                 (cudaStream_t)stream, RopeTable{nullptr, nullptr, 0}, &da));
   const krill_status_t st = do_attention(p, n_seqs, seqs, layer_begin, layer_count, q, q_dtype, out,
@@ -1580,7 +1907,10 @@ krill_status_t krill_decode_step(krill_pool_t p, int32_t n_seqs, const krill_seq
     flush_deferred_append(p, da, (cudaStream_t)stream);
     if (st != KRILL_OK) set_error(st, msg.c_str());
   }
-  return st;
+  if (st == KRILL_OK) return run_deferred_summaries(p, da, (cudaStream_t)stream);
+  const std::string msg = krill_last_error_string();
+  run_deferred_summaries(p, da, (cudaStream_t)stream);  // the tokens are in place all the same
+  return set_error(st, msg.c_str());
 }
 
 krill_status_t krill_decode_step_host(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs,
@@ -1672,6 +2002,7 @@ krill_status_t krill_decode_step_host(krill_pool_t p, int32_t n_seqs, const kril
     // as krill_decode_step: the append rides in the attention's packet
     DeferredAppend& da = p->deferred;
     da.pending = false;
+    da.sums.clear();
     rc = do_append(p, n_seqs, seqs, layer_begin + (int32_t)c0, lc, 1, d + k_off + c0 * kv_l,
                    d + v_off + c0 * kv_l, kv_dtype, s, RopeTable{nullptr, nullptr, 0}, &da);
     if (rc == KRILL_OK)
@@ -1683,6 +2014,13 @@ krill_status_t krill_decode_step_host(krill_pool_t p, int32_t n_seqs, const kril
       flush_deferred_append(p, da, s);
       if (rc != KRILL_OK) set_error(rc, msg.c_str());
     }
+    if (rc != KRILL_OK) {
+      const std::string msg = krill_last_error_string();
+      run_deferred_summaries(p, da, s);
+      set_error(rc, msg.c_str());
+      break;
+    }
+    rc = run_deferred_summaries(p, da, s);
     if (rc != KRILL_OK) break;
     if (c + 1 < n_ch) {
       rc = copy_in(c + 1);
@@ -1708,7 +2046,7 @@ krill_status_t krill_seq_snapshot_quantized(krill_pool_t p, krill_seq_t h, int32
                                             void* value_zeros, void* stream) {
   if (!p) return fail(KRILL_ERR_INVALID, "null pool");
   std::lock_guard<std::recursive_mutex> lk(p->mu);
-  if (p->geom.fmt != kFmtInt8) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 pool");
+  if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 or 4-bit pool");
   TRY(require_device(p));
   DeviceGuard dg(p->device);
   Seq* s = nullptr;
@@ -1739,7 +2077,7 @@ krill_status_t krill_seq_snapshot_dequantized(krill_pool_t p, krill_seq_t h, int
                                               void* keys, void* values, void* stream) {
   if (!p) return fail(KRILL_ERR_INVALID, "null pool");
   std::lock_guard<std::recursive_mutex> lk(p->mu);
-  if (p->geom.fmt != kFmtInt8) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 pool");
+  if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 or 4-bit pool");
   TRY(require_device(p));
   DeviceGuard dg(p->device);
   Seq* s = nullptr;
@@ -1768,7 +2106,7 @@ krill_status_t krill_seq_restore_quantized(krill_pool_t p, krill_seq_t h, int32_
                                            const void* value_zeros, void* stream) {
   if (!p) return fail(KRILL_ERR_INVALID, "null pool");
   std::lock_guard<std::recursive_mutex> lk(p->mu);
-  if (p->geom.fmt != kFmtInt8) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 pool");
+  if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 or 4-bit pool");
   DeviceGuard dg(p->device);
   Seq* s = nullptr;
   TRY(seq_get(p, h, &s));
@@ -1791,7 +2129,7 @@ krill_status_t krill_stack_left_padded(krill_pool_t p, int32_t n_seqs, const kri
                                        void* value_zeros, void* stream) {
   if (!p) return fail(KRILL_ERR_INVALID, "null pool");
   std::lock_guard<std::recursive_mutex> lk(p->mu);
-  if (p->geom.fmt != kFmtInt8) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 pool");
+  if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 or 4-bit pool");
   TRY(require_device(p));
   DeviceGuard dg(p->device);
   if (layer < 0 || layer >= p->geom.L) return fail(KRILL_ERR_INVALID, "bad layer");
@@ -1843,7 +2181,7 @@ krill_status_t krill_scatter_back(krill_pool_t p, int32_t n_seqs, const krill_se
                                   void* stream) {
   if (!p) return fail(KRILL_ERR_INVALID, "null pool");
   std::lock_guard<std::recursive_mutex> lk(p->mu);
-  if (p->geom.fmt != kFmtInt8) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 pool");
+  if (p->geom.fmt == kFmtBf16) return fail(KRILL_ERR_INVALID, "quantized snapshots need an int8 or 4-bit pool");
   TRY(require_device(p));
   DeviceGuard dg(p->device);
   if (layer < 0 || layer >= p->geom.L) return fail(KRILL_ERR_INVALID, "bad layer");
@@ -2739,8 +3077,8 @@ krill_status_t krill_prefix_peer_fetch(krill_prefix_t dst, krill_prefix_t src,
   krill_pool_t dp = dst->pool, sp = src->pool;
   if (dp->host_only || sp->host_only) return fail(KRILL_ERR_NO_DEVICE, "peer fetch needs device pools");
   const Geom &a = dp->geom, &b = sp->geom;
-  if (a.L != b.L || a.Hkv != b.Hkv || a.D != b.D || a.G != b.G || a.ring != b.ring ||
-      dp->cfg.window != sp->cfg.window)
+  if (a.L != b.L || a.Hkv != b.Hkv || a.D != b.D || a.G != b.G || a.ring != b.ring || a.fmt != b.fmt ||
+      a.block_bytes != b.block_bytes || dp->cfg.window != sp->cfg.window)
     return fail(KRILL_ERR_INVALID, "peer fetch between pools of different geometry");
   auto* e = new krill_prefix_entry_s();
   {

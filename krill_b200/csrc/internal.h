@@ -140,6 +140,10 @@ struct AttnParams {
   int sh_grid;                // CTAs, or CTA pairs when sh_pair (sh_cta_off per pair)
   int sh_pair;                // 1: the tcgen05 cascade runs as CTA pairs (cta_group::2)
   int n_pslots;               // prefix record slots per cascaded unit
+  // Block-sparse decode: the picked sub-blocks of (unit, kv head), ascending,
+  // [units][Hkv][sel_stride]; unit items then index this list. nullptr: dense.
+  const int32_t* sel;
+  int sel_stride;
   // host side only: launch the decode kernel as the programmatic dependent of
   // the append kernel launched just before it on the stream
   int pdl;
@@ -166,6 +170,45 @@ inline int append_tile_chunks(int n_new, int subt) { return (n_new + subt - 1) /
 cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin,
                           int layer_count, int n_seqs, int n_new, const void* k, const void* v,
                           int dtype, int* large_scale, RopeTable rope, cudaStream_t stream);
+// The same for 4-bit pools (kv_int4.cu).
+cudaError_t launch_append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin, int layer_count,
+                           int n_seqs, int n_new, const void* k, const void* v, int dtype, int* large_scale,
+                           RopeTable rope, cudaStream_t stream);
+cudaError_t launch_gather4(const Geom& g, const uint8_t* pool, int layer, const int32_t* d_bt, int64_t p0,
+                           int64_t S, const GatherOut& out, cudaStream_t stream);
+cudaError_t launch_scatter4(const Geom& g, uint8_t* pool, int layer, const int32_t* d_bt, int64_t p0, int64_t S,
+                            const ScatterIn& in, int* large_scale, cudaStream_t stream);
+// Dequantized rows [starts[si], + n) of (layers x sequences) of an int8 or
+// 4-bit pool, laid out like an append's input (kv_int4.cu).
+cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const int32_t* d_bt, int bt_stride,
+                             const int64_t* d_starts, int layer_begin, int layer_count, int n_seqs, int64_t n,
+                             void* keys, void* values, int dtype, cudaStream_t stream);
+
+// One sub-block whose summary is to be computed, for every kv head.
+struct SumItem {
+  int32_t block, layer, sub;
+};
+// Block choice (kv_select.cu): per (unit, kv head) the budget best sub-blocks.
+struct SelectParams {
+  const uint8_t* pool;
+  int64_t page_bytes, sum_off;
+  int L, Hkv, Hq, g, spb, T;
+  const AttnUnit* units;
+  const int32_t* bt;
+  int bt_stride;
+  const void* q;
+  int q_dtype;
+  int budget, first, last;  // first / last blocks are always picked; budget >= first + last
+  int32_t* sel;             // [units][Hkv][budget], -1 past the last
+  uint32_t* scratch;        // keys [units * Hkv][scratch_stride], or nullptr: shared memory
+  int64_t scratch_stride;
+};
+// Most blocks of one sequence whose keys are kept in shared memory.
+constexpr int64_t kSelectSmemKeys = 49152;
+cudaError_t launch_summaries(const Geom& g, uint8_t* pool, const SumItem* d_items, int64_t n_items,
+                             cudaStream_t stream);
+cudaError_t launch_select(const Geom& g, const SelectParams& p, int n_units, int64_t max_n, int num_sms,
+                          cudaStream_t stream);
 cudaError_t launch_gather(const Geom& g, const uint8_t* pool, int layer, const int32_t* d_bt,
                           int64_t p0, int64_t S, const GatherOut& out, cudaStream_t stream);
 cudaError_t launch_scatter(const Geom& g, uint8_t* pool, int layer, const int32_t* d_bt, int64_t p0,
@@ -181,6 +224,11 @@ void describe_attention(const Geom& g, const AttnParams& p, int grid, int impl, 
 cudaError_t launch_shared(const Geom& g, const AttnParams& p, cudaStream_t stream);
 // Merge the partial records of p.split_units (attn_combine_kernel) on its own.
 cudaError_t launch_combine(const Geom& g, const AttnParams& p, cudaStream_t stream);
+// launch_attention's decode kernel for 4-bit pools (kv_attn4.cu) and for
+// picked blocks (p.sel) of int8 pools (kv_attn_sel.cu).
+cudaError_t launch_attention4(const Geom& g, const AttnParams& p, int grid, cudaStream_t stream);
+cudaError_t launch_attention_sel8(const Geom& g, const AttnParams& p, int grid, cudaStream_t stream);
+int describe_attention4(const Geom& g, const AttnParams& p, char* buf, size_t cap);
 // True when launch_attention runs the combine kernel: split units whose records
 // are not merged by the last-arriving decode piece (no counters, no decode
 // kernel, or the CUDA-core variant).

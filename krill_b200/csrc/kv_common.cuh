@@ -21,6 +21,25 @@
 //                          rows swapped pairwise (chunk ^ 1) so the decode
 //                          kernel's shared-memory reads are conflict free
 //     [2*T*D, 4*T*D)       V transposed: D rows of T bf16
+//
+// 4-bit pools use sub-blocks of T = 64 tokens of T * (D + 8*NG) bytes:
+//     [0, 32*D)            K codes in the order of the decode kernel's MMA
+//                          operand: 16-token x 16-element tiles of 32 lane
+//                          words, the four tiles of 64 elements interleaved so
+//                          that one 16-byte load per lane fetches them. Byte
+//                          (2h + hi) of word k holds the codes d (low nibble)
+//                          and d + 2 (high) of one token, d = 16c + 4k + h
+//     [32*D, 64*D)         V codes, tiles of 16 elements x 16 tokens, the four
+//                          token tiles interleaved; a byte holds the codes d
+//                          and d + 8 of one token
+//     [64*D, ...)          K scales, K zeros, V scales, V zeros: [NG][T] f16,
+//                          token t at (t % 8) * 8 + t / 8, so that the eight
+//                          tokens of one operand row are 16 consecutive bytes
+// Every code byte belongs to one token, so tokens are written independently.
+//
+// A pool with block summaries ends each page with spb rows of 2*D bytes (per
+// K channel of the sub-block: mid, then half-range, as int8 in units of
+// sigma) followed by spb f32 sigmas, padded to 16 bytes.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,6 +55,9 @@ __host__ __device__ constexpr int sub_tokens_raw(int D) { return D >= 128 ? 32 :
 // Pool formats.
 constexpr int kFmtInt8 = 0;
 constexpr int kFmtBf16 = 1;
+constexpr int kFmtInt4 = 2;
+// Tokens per sub-block of a 4-bit pool.
+constexpr int kSub4 = 64;
 
 struct Geom {
   int L;        // layers in the pool
@@ -48,23 +70,33 @@ struct Geom {
   int ring;     // blocks in a windowed sequence's ring; 0 = full history
   int window;   // sliding window (tokens); 0 = full history
   int quant_variant;
-  int fmt;      // kFmtInt8 or kFmtBf16
+  int fmt;      // kFmtInt8, kFmtBf16 or kFmtInt4
   int subt;     // tokens per sub-block
   int spb;      // sub-blocks per 256-token block
   int64_t sb_bytes;
+  int64_t sum_off;  // byte offset of a page's block summaries; 0 = none
   int64_t page_bytes;
   int64_t block_bytes;
 };
 
+// Bytes of a page's block summaries (spb sub-blocks).
+__host__ __device__ inline int64_t summary_bytes(int D, int spb) {
+  return ((int64_t)spb * (2 * D + 4) + 15) / 16 * 16;
+}
+
 inline Geom make_geom(int L, int Hkv, int Hq, int D, int G, int ring, int window, int qv,
-                      int fmt = kFmtInt8) {
+                      int fmt = kFmtInt8, bool summaries = false) {
   Geom g;
   g.L = L; g.Hkv = Hkv; g.Hq = Hq; g.g = Hq / Hkv; g.D = D; g.G = G; g.NG = D / G;
   g.ring = ring; g.window = window; g.quant_variant = qv; g.fmt = fmt;
-  g.subt = fmt == kFmtBf16 ? sub_tokens_raw(D) : sub_tokens(D);
+  g.subt = fmt == kFmtBf16 ? sub_tokens_raw(D) : fmt == kFmtInt4 ? kSub4 : sub_tokens(D);
   g.spb = kBlockTokens / g.subt;
-  g.sb_bytes = fmt == kFmtBf16 ? (int64_t)g.subt * 4 * D : (int64_t)g.subt * (2 * D + 8 * g.NG);
+  g.sb_bytes = fmt == kFmtBf16   ? (int64_t)g.subt * 4 * D
+               : fmt == kFmtInt4 ? (int64_t)g.subt * (D + 8 * g.NG)
+                                 : (int64_t)g.subt * (2 * D + 8 * g.NG);
   g.page_bytes = g.sb_bytes * g.spb;
+  g.sum_off = summaries ? g.page_bytes : 0;
+  if (summaries) g.page_bytes += summary_bytes(D, g.spb);
   g.block_bytes = g.page_bytes * L * Hkv;
   return g;
 }
@@ -94,6 +126,24 @@ __host__ __device__ inline int64_t raw_koff(int D, int t, int d) {
 __host__ __device__ inline int64_t raw_voff(int D, int T, int t, int d) {
   return ((int64_t)T * D + (int64_t)d * T + t) * 2;
 }
+
+// 4-bit sub-block: byte j (0..7) of 16-element chunk c of token t. K: codes
+// d = 16c + 4(j/2) + j%2 (low nibble) and d + 2; V: codes d = 16c + j and d + 8.
+__host__ __device__ inline int q4_kbyte(int D, int t, int c, int j) {
+  return ((((t >> 4) * (D >> 6) + (c >> 2)) * 32 + (t & 7) * 4 + (c & 3)) << 4) + (j >> 1) * 4 + (j & 1) * 2 +
+         ((t >> 3) & 1);
+}
+__host__ __device__ inline int q4_vbyte(int D, int t, int c, int j) {
+  return 32 * D + ((c * 32 + j * 4 + ((t & 7) >> 1)) << 4) + (t >> 4) * 4 + (t & 1) * 2 + ((t >> 3) & 1);
+}
+// meta array a (0 = K scale, 1 = K zero, 2 = V scale, 3 = V zero), group gi, token t
+__host__ __device__ inline int q4_meta(int D, int NG, int a, int gi, int t) {
+  return kSub4 * D + ((a * NG + gi) * kSub4 + (t & 7) * 8 + (t >> 3)) * 2;
+}
+// Element of a 4-bit chunk held in the low nibble of its byte j, and the
+// distance to the one in the high nibble.
+__host__ __device__ constexpr int q4_elem(bool is_k, int j) { return is_k ? 4 * (j >> 1) + (j & 1) : j; }
+__host__ __device__ constexpr int q4_step(bool is_k) { return is_k ? 2 : 8; }
 
 // Error flag bits written by kernels (pool-owned int, read + cleared by host).
 constexpr int kErrTimeout = 1;

@@ -121,13 +121,15 @@ __device__ __forceinline__ uint32_t neg1024(uint32_t s2) {
 template <int D, int NG, int FMT = kFmtInt8>
 struct SubGeom {
   static constexpr int G = D / NG;
-  static constexpr int T = FMT == kFmtBf16 ? sub_tokens_raw(D) : sub_tokens(D);
+  static constexpr int T = FMT == kFmtBf16 ? sub_tokens_raw(D) : FMT == kFmtInt4 ? kSub4 : sub_tokens(D);
   static constexpr int SPB = kBlockTokens / T;
   static constexpr int NU = T / 16;          // 16-token m-tiles per sub-block
   static constexpr int TPT = T / 4;          // tokens per lane chunk (V rows)
-  static constexpr int SB = FMT == kFmtBf16 ? T * 4 * D : T * (2 * D + 8 * NG);
-  static constexpr int VOFF = FMT == kFmtBf16 ? T * D * 2 : T * D;
-  static constexpr int META = 2 * T * D;     // int8 only
+  static constexpr int SB = FMT == kFmtBf16   ? T * 4 * D
+                            : FMT == kFmtInt4 ? T * (D + 8 * NG)
+                                              : T * (2 * D + 8 * NG);
+  static constexpr int VOFF = FMT == kFmtBf16 ? T * D * 2 : FMT == kFmtInt4 ? T * D / 2 : T * D;
+  static constexpr int META = FMT == kFmtInt4 ? T * D : 2 * T * D;  // int8 and int4
   // meta array a, group gi, token t -> byte offset (int8 only)
   static __device__ __forceinline__ int meta(int a, int gi, int t) {
     return META + ((a * NG + gi) * T + t) * 2;
@@ -136,6 +138,13 @@ struct SubGeom {
 
 __device__ __forceinline__ uint32_t f2h2(float lo, float hi) {
   return h2u(__floats2half2_rn(lo, hi));
+}
+// 2^x by the special-function unit (ex2.approx.ftz.f32: one instruction;
+// results below 2^-126 flush to zero, immaterial next to a row sum >= 1).
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // bf16 pair -> f16 pair; exact for magnitudes in the f16 normal range
 __device__ __forceinline__ uint32_t bf2h2(uint32_t w) {

@@ -648,6 +648,9 @@ cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, 
                           int dtype, int* large_scale, RopeTable rope, cudaStream_t stream) {
   const int64_t warps = (int64_t)layer_count * n_seqs * g.Hkv * n_new;
   if (warps == 0) return cudaSuccess;
+  if (g.fmt == kFmtInt4)
+    return launch_append4(g, pool, d_dst, layer_begin, layer_count, n_seqs, n_new, k, v, dtype, large_scale, rope,
+                          stream);
   const int threads = 256;
   const int64_t blocks = (warps * 32 + threads - 1) / threads;
   if (g.fmt == kFmtBf16) {
@@ -740,6 +743,7 @@ cudaError_t launch_gather(const Geom& g, const uint8_t* pool, int layer, const i
                           int64_t p0, int64_t S, const GatherOut& out, cudaStream_t stream) {
   const int64_t total = (int64_t)g.Hkv * S * (g.D / 8);
   if (total == 0) return cudaSuccess;
+  if (g.fmt == kFmtInt4) return launch_gather4(g, pool, layer, d_bt, p0, S, out, stream);
   const int threads = 256;
   gather_kernel<<<(unsigned)((total + threads - 1) / threads), threads, 0, stream>>>(pool, g, layer,
                                                                                      d_bt, p0, S, out);
@@ -750,6 +754,7 @@ cudaError_t launch_scatter(const Geom& g, uint8_t* pool, int layer, const int32_
                            int64_t S, const ScatterIn& in, int* large_scale, cudaStream_t stream) {
   const int64_t total = (int64_t)g.Hkv * S * (g.D / 8);
   if (total == 0) return cudaSuccess;
+  if (g.fmt == kFmtInt4) return launch_scatter4(g, pool, layer, d_bt, p0, S, in, large_scale, stream);
   const int threads = 256;
   scatter_kernel<<<(unsigned)((total + threads - 1) / threads), threads, 0, stream>>>(
       pool, g, layer, d_bt, p0, S, in, large_scale);

@@ -7,8 +7,8 @@
 // rows as two 128-row halves that share every K/V tile. One CTA per SM, 20
 // warps:
 //   - warp 9 streams raw sub-blocks HBM -> shared memory (cp.async.bulk);
-//   - warps 10-19 dequantize each raw sub-block once (the reference's two
-//     fp16 roundings) into f16 K [64 tok][D] and V [D][64 tok] tiles laid out
+//   - warps 10-19 dequantize each raw sub-block once (int8: the reference's two
+//     fp16 roundings; 4-bit pools: one fma) into f16 K [64 tok][D] and V [D][64 tok] tiles laid out
 //     as the tensor core's canonical K-major 128-byte-swizzled operands;
 //   - warp 8 owns the tensor memory (512 columns) and one of its lanes issues
 //     the MMAs, per half h:
@@ -148,9 +148,9 @@ __device__ __forceinline__ uint32_t sw128_off(int rows, int r, int c) {
 }
 
 
-template <int D, int NG>
+template <int D, int NG, int FMT>
 struct UmSmem {
-  using SG = SubGeom<D, NG>;
+  using SG = SubGeom<D, NG, FMT>;
   static_assert(SG::T == 64, "one 64-token sub-block per tile");
   static constexpr int QH_BYTES = 128 * D * 2;  // one 128-row half of the Q tile
   static constexpr int P_BYTES = 128 * 64 * 2;  // one half's P tile
@@ -269,12 +269,76 @@ __device__ __forceinline__ void um_dequant(const uint8_t* __restrict__ raw, uint
   }
 }
 
-// 2^x by the special-function unit (ex2.approx.ftz.f32: one instruction;
-// results below 2^-126 flush to zero, immaterial next to a row sum >= 1).
-__device__ __forceinline__ float ex2_ftz(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// um_dequant for 4-bit pools: values f16(code * scale + zero), one fma per
+// pair. A K item is a lane word group of the sub-block (tokens r and r + 8, 16
+// elements each, in order), a V item one of four token tiles (two rows d, d +
+// 8, pairs of tokens). Tokens at or past `valid` read as zero, whatever the
+// sub-block holds there.
+__device__ __forceinline__ uint32_t deq4(uint32_t w, uint32_t s2, uint32_t z2) {
+  const __half2 c = __hsub2_rn(u2h((w & 0x000f000fu) | 0x64006400u), u2h(0x64006400u));  // 1024 + c - 1024
+  return h2u(__hfma2(c, u2h(s2), u2h(z2)));
+}
+template <int D, int NG>
+__device__ __forceinline__ void um_dequant4(const uint8_t* __restrict__ raw, uint8_t* __restrict__ kt,
+                                            uint8_t* __restrict__ vt, int t0, int valid) {
+  using SG = SubGeom<D, NG, kFmtInt4>;
+  constexpr int NDT = kUmDeqWarps * 32, NHH = D / 64, NK = 4 * NHH * 32, NV = D / 16 * 32;
+  const uint8_t* meta = raw + SG::META;
+  for (int i = t0; i < NK + NV; i += NDT) {
+    const int lane = i & 31, r = lane >> 2, tig = lane & 3;
+    if (i < NK) {
+      const int hh = (i >> 5) % NHH, u = (i >> 5) / NHH, grp = 64 * hh / SG::G, t = 16 * u + r;
+      const uint4 w4 = *reinterpret_cast<const uint4*>(raw + i * 16);
+      uint32_t s = *reinterpret_cast<const uint32_t*>(meta + grp * 128 + r * 16 + 4 * u);  // tokens t, t + 8
+      uint32_t z = *reinterpret_cast<const uint32_t*>(meta + (NG + grp) * 128 + r * 16 + 4 * u);
+      if (valid < 64) {
+        const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 8 < valid ? 0xffff0000u : 0u);
+        s &= mk;
+        z &= mk;
+      }
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const uint32_t s2 = __byte_perm(s, 0, hi ? 0x3232 : 0x1010), z2 = __byte_perm(z, 0, hi ? 0x3232 : 0x1010);
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = deq4(w[k] >> (8 * hi), s2, z2);
+          o[2 * k + 1] = deq4(w[k] >> (8 * hi + 4), s2, z2);
+        }
+        const int c = 2 * (4 * hh + tig);
+        *reinterpret_cast<uint4*>(kt + sw128_off(64, t + 8 * hi, c)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(kt + sw128_off(64, t + 8 * hi, c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    } else {
+      const int v = i - NK, mt = v >> 5, grp = 16 * mt / SG::G, d = 16 * mt + r;
+      const uint4 w4 = *reinterpret_cast<const uint4*>(raw + SG::VOFF + v * 16);
+      // scales / zeros of the tokens 16u + 8hi + 2 tig (a) and + 1 (b)
+      const uint4 sa4 = *reinterpret_cast<const uint4*>(meta + (2 * NG + grp) * 128 + 32 * tig);
+      const uint4 sb4 = *reinterpret_cast<const uint4*>(meta + (2 * NG + grp) * 128 + 32 * tig + 16);
+      const uint4 za4 = *reinterpret_cast<const uint4*>(meta + (3 * NG + grp) * 128 + 32 * tig);
+      const uint4 zb4 = *reinterpret_cast<const uint4*>(meta + (3 * NG + grp) * 128 + 32 * tig + 16);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      const uint32_t sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w}, sb[4] = {sb4.x, sb4.y, sb4.z, sb4.w};
+      const uint32_t za[4] = {za4.x, za4.y, za4.z, za4.w}, zb[4] = {zb4.x, zb4.y, zb4.z, zb4.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+          uint32_t s2 = __byte_perm(sa[u], sb[u], hi ? 0x7632 : 0x5410);
+          uint32_t z2 = __byte_perm(za[u], zb[u], hi ? 0x7632 : 0x5410);
+          if (valid < 64) {
+            const int t = 16 * u + 8 * hi + 2 * tig;
+            const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 1 < valid ? 0xffff0000u : 0u);
+            s2 &= mk;
+            z2 &= mk;
+          }
+          *reinterpret_cast<uint32_t*>(vt + sw128_off(D, d, 2 * u + hi) + 4 * tig) = deq4(w[u] >> (8 * hi), s2, z2);
+          *reinterpret_cast<uint32_t*>(vt + sw128_off(D, d + 8, 2 * u + hi) + 4 * tig) =
+              deq4(w[u] >> (8 * hi + 4), s2, z2);
+        }
+    }
+  }
 }
 
 __device__ __forceinline__ float max64(const float (&a)[32], const float (&b)[32]) {
@@ -288,10 +352,10 @@ __device__ __forceinline__ float max64(const float (&a)[32], const float (&b)[32
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-template <int D, int NG>
+template <int D, int NG, int FMT>
 __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnParams p) {
-  using SM = UmSmem<D, NG>;
-  using SG = SubGeom<D, NG>;
+  using SM = UmSmem<D, NG, FMT>;
+  using SG = SubGeom<D, NG, FMT>;
   constexpr int SB = SG::SB;
   extern __shared__ __align__(1024) uint8_t smem[];
   // The swizzled operand tiles need 1024-byte alignment. The dynamic shared
@@ -379,7 +443,11 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
         if (J >= (uint32_t)kUmNF)
           mbar_wait(bar(SM::B_KE + fs), ((J / kUmNF) - 1) & 1, cta_abort, p.err);
         uint8_t* kt = smem + SM::KV_OFF + fs * SM::KV_STAGE;
-        um_dequant<D, NG>(smem + SM::RAW_OFF + rs * SB, kt, kt + SM::K_BYTES, t0);
+        if constexpr (FMT == kFmtInt4)  // tokens past the last query's position count as zero
+          um_dequant4<D, NG>(smem + SM::RAW_OFF + rs * SB, kt, kt + SM::K_BYTES, t0,
+                             item.causal < 0 ? 64 : item.causal + (item.n_rows - 1) / p.g + 1 - 64 * j);
+        else
+          um_dequant<D, NG>(smem + SM::RAW_OFF + rs * SB, kt, kt + SM::K_BYTES, t0);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -665,9 +733,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
   }
 }
 
-template <int D, int NG>
+template <int D, int NG, int FMT = kFmtInt8>
 cudaError_t launch_um(const AttnParams& p, cudaStream_t stream) {
-  using SM = UmSmem<D, NG>;
+  using SM = UmSmem<D, NG, FMT>;
   static_assert(SM::TOTAL <= 232448, "shared memory budget");
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
@@ -678,16 +746,16 @@ cudaError_t launch_um(const AttnParams& p, cudaStream_t stream) {
     // setmaxnreg.inc waits until the released registers cover it: refuse to
     // launch a build whose register count would not balance
     cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, attn_shared_umma_kernel<D, NG>);
+    e = cudaFuncGetAttributes(&fa, attn_shared_umma_kernel<D, NG, FMT>);
     if (e != cudaSuccess) return e;
     if (fa.numRegs * kUmThreads < 256 * kUmSoftmaxRegs + (kUmThreads - 256) * kUmOtherRegs)
       return cudaErrorInvalidConfiguration;
-    e = cudaFuncSetAttribute(attn_shared_umma_kernel<D, NG>,
+    e = cudaFuncSetAttribute(attn_shared_umma_kernel<D, NG, FMT>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit);
   }
-  attn_shared_umma_kernel<D, NG><<<p.sh_grid, kUmThreads, SM::TOTAL, stream>>>(p);
+  attn_shared_umma_kernel<D, NG, FMT><<<p.sh_grid, kUmThreads, SM::TOTAL, stream>>>(p);
   return cudaGetLastError();
 }
 
@@ -1350,6 +1418,12 @@ cudaError_t launch_shared_umma(const Geom& g, const AttnParams& p, cudaStream_t 
     if (g.D == 64 && g.NG == 1) return launch_pair<64, 1>(p, stream);
     if (g.D == 128 && g.NG == 2) return launch_pair<128, 2>(p, stream);
     if (g.D == 128 && g.NG == 1) return launch_pair<128, 1>(p, stream);
+    return cudaErrorInvalidValue;
+  }
+  if (g.fmt == kFmtInt4) {
+    if (g.D == 64 && g.NG == 1) return launch_um<64, 1, kFmtInt4>(p, stream);
+    if (g.D == 128 && g.NG == 2) return launch_um<128, 2, kFmtInt4>(p, stream);
+    if (g.D == 128 && g.NG == 1) return launch_um<128, 1, kFmtInt4>(p, stream);
     return cudaErrorInvalidValue;
   }
   if (g.D == 64 && g.NG == 1) return launch_um<64, 1>(p, stream);
