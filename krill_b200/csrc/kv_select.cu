@@ -125,14 +125,16 @@ __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __r
   if (tid == 0) *reinterpret_cast<float*>(page + geom.sum_off + (int64_t)geom.spb * 2 * D + 4 * it.sub) = sigma;
 }
 
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;
+constexpr int kRegKeys = 16;             // keys a thread holds while it picks
 constexpr uint32_t kForced = 0xffffffffu;  // above the key of every score
 
-// Order-preserving key of a score (equal scores, +-0 included, get equal keys).
+// Order-preserving key of a score, at least 1 (equal scores, +-0 included, get
+// equal keys).
 __device__ __forceinline__ uint32_t score_key(float x) {
   const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
-  if (isnan(x)) return 0u;
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  if (isnan(x)) return 1u;
+  return (b & 0x80000000u) ? max(~b, 1u) : (b | 0x80000000u);
 }
 
 __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -142,27 +144,171 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+struct PickSmem {
+  uint32_t red[2][kSelWarps];          // double-buffered block reductions
+  uint32_t cnt[kRegKeys][kSelWarps];   // per key round and warp: picked-for-sure | equal << 16
+};
+
+// Sum / min / max over the NW warps that pick (one: no barrier).
+template <int NW, typename F>
+__device__ __forceinline__ uint32_t pick_reduce(uint32_t x, PickSmem& sm, int& buf, int warp, int lane, F op) {
+  if (NW == 1) return x;
+  if (lane == 0) sm.red[buf][warp] = x;
+  __syncthreads();
+  x = sm.red[buf][0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) x = op(x, sm.red[buf][w]);
+  buf ^= 1;
+  return x;
+}
+
+// The `want` largest keys (equal ones: the first) besides the forced ones, at
+// most kRegKeys * 32 * NW of them, by bisection over the bits in which the keys
+// differ, each thread holding its keys in registers; their indices to `out` in
+// order. NW warps call it.
+template <int NW>
+__device__ __forceinline__ void pick_in_registers(const uint32_t* keys, int n, int want, int32_t* out, PickSmem& sm,
+                                                  int warp, int lane) {
+  constexpr int STEP = 32 * NW;
+  const int at = warp * 32 + lane, rounds = (n + STEP - 1) / STEP;
+  uint32_t k[kRegKeys], lo = 0xffffffffu, hi = 0u;
+  int buf = 0;
+#pragma unroll
+  for (int j = 0; j < kRegKeys; ++j) {
+    k[j] = 0u;
+    if (j < rounds) {
+      if (at + j * STEP < n) k[j] = keys[at + j * STEP];
+      if (k[j] != 0u && k[j] != kForced) {
+        lo = min(lo, k[j]);
+        hi = max(hi, k[j]);
+      }
+    }
+  }
+  lo = pick_reduce<NW>(__reduce_min_sync(0xffffffffu, lo), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return min(a, b); });
+  hi = pick_reduce<NW>(__reduce_max_sync(0xffffffffu, hi), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return max(a, b); });
+  // K: the largest threshold with at least `want` keys in [K, kForced)
+  uint32_t K = kForced - 1u;
+  int above = 0;
+  if (want > 0) {
+    const int top = 32 - __clz(lo ^ hi);  // bits that differ
+    K = top >= 32 ? 0u : lo >> top << top;
+    for (int bit = top - 1; bit >= 0; --bit) {
+      const uint32_t cand = K | (1u << bit);
+      uint32_t c = 0;
+#pragma unroll
+      for (int j = 0; j < kRegKeys; ++j)
+        if (j < rounds) c += k[j] >= cand && k[j] != kForced ? 1u : 0u;
+      c = pick_reduce<NW>(__reduce_add_sync(0xffffffffu, c), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return a + b; });
+      if ((int)c >= want) K = cand;
+      if ((int)c == want) break;  // exactly the keys from K on
+    }
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < kRegKeys; ++j)
+      if (j < rounds) c += k[j] > K && k[j] != kForced ? 1u : 0u;
+    above = (int)pick_reduce<NW>(__reduce_add_sync(0xffffffffu, c), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return a + b; });
+  }
+  const int need = want - above;  // of the keys equal to K, the first ones
+  // positions: keys above K (forced ones among them) before, and equal ones
+  uint32_t mg[kRegKeys], me[kRegKeys];
+#pragma unroll
+  for (int j = 0; j < kRegKeys; ++j)
+    if (j < rounds) {
+      mg[j] = __ballot_sync(0xffffffffu, k[j] > K);
+      me[j] = __ballot_sync(0xffffffffu, k[j] == K && K != 0u);
+      if (NW > 1 && lane == 0) sm.cnt[j][warp] = __popc(mg[j]) | (__popc(me[j]) << 16);
+    }
+  if (NW > 1) __syncthreads();
+  const uint32_t below = (1u << lane) - 1u;
+  int g0 = 0, e0 = 0;
+#pragma unroll
+  for (int j = 0; j < kRegKeys; ++j)
+    if (j < rounds) {
+      int gb = g0, eb = e0;
+      if (NW == 1) {
+        g0 += __popc(mg[j]);
+        e0 += __popc(me[j]);
+      } else {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const uint32_t c = sm.cnt[j][w];
+          if (w < warp) {
+            gb += c & 0xffff;
+            eb += c >> 16;
+          }
+          g0 += c & 0xffff;
+          e0 += c >> 16;
+        }
+      }
+      gb += __popc(mg[j] & below);
+      eb += __popc(me[j] & below);
+      const bool gt = (mg[j] >> lane) & 1u, eq = (me[j] >> lane) & 1u;
+      if (gt || (eq && eb < need)) out[gb + min(eb, need)] = at + j * STEP;
+    }
+}
+
+// The same for any number of keys, read again in every round.
+__device__ __forceinline__ void pick_in_memory(const uint32_t* keys, int n, int budget, int32_t* out, PickSmem& sm,
+                                               int tid, int warp, int lane) {
+  int buf = 0;
+  auto add = [](uint32_t a, uint32_t b) { return a + b; };
+  auto count = [&](uint32_t from) {
+    uint32_t c = 0;
+    for (int i = tid; i < n; i += kSelThreads) c += keys[i] >= from ? 1u : 0u;
+    return (int)pick_reduce<kSelWarps>(__reduce_add_sync(0xffffffffu, c), sm, buf, warp, lane, add);
+  };
+  uint32_t K = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cand = K | (1u << bit);
+    if (count(cand) >= budget) K = cand;
+  }
+  const int need = budget - (K == kForced ? 0 : count(K + 1u));
+  int gt_before = 0, eq_before = 0;
+  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
+    const int i = i0 + tid;
+    const uint32_t k = i < n ? keys[i] : 0u;
+    const bool gt = i < n && k > K, eq = i < n && k == K;
+    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+    if (lane == 0) sm.red[buf][warp] = __popc(mg) | (__popc(me) << 16);
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kSelWarps; ++w) {
+      if (w < warp) before += sm.red[buf][w];
+      total += sm.red[buf][w];
+    }
+    const uint32_t below = (1u << lane) - 1u;
+    const int gb = gt_before + (before & 0xffff) + __popc(mg & below);
+    const int eb = eq_before + (before >> 16) + __popc(me & below);
+    if (gt || (eq && eb < need)) out[gb + min(eb, need)] = i;
+    gt_before += total & 0xffff;
+    eq_before += total >> 16;
+    buf ^= 1;
+  }
+}
+
 // One cluster of CTAs per (unit, kv head). The cluster's warps score 16 blocks
 // at a time against the head's (at most 8) query heads in one chain of int8
 // MMAs (rows = blocks, columns = query heads, K = the 2 D summary bytes; the
 // byte order along K is permuted alike on both sides, so that a lane's operand
-// is 16 consecutive bytes), the keys go to the first CTA's shared memory (or
-// to scratch, for sequences of more blocks than fit), and that CTA finds the
-// n_sel-th largest key by bisection over its bits and writes the picked
-// indices in order.
+// is 16 consecutive bytes); the keys go to the first CTA's shared memory (or
+// to scratch, for sequences of more blocks than fit), which picks: up to 512
+// blocks in one warp without barriers, up to 2048 in four, more by reading the
+// keys again for each bit.
 template <int D>
 __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ uint32_t keys_smem[];
   __shared__ __align__(16) int8_t qa[8][2 * D];
   __shared__ float tau_s[8];
-  __shared__ int cnt_s[2][kSelThreads / 32];
+  __shared__ PickSmem sm;
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int uid = blockIdx.x / CL, ui = uid / p.Hkv, h = uid % p.Hkv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const AttnUnit un = p.units[ui];
-  const int n = (un.t_hi + p.T - 1) / p.T;
+  const AttnUnit* unit = p.units + ui;
+  const int si = unit->si, layer = unit->layer, qo_row = unit->qo_row;
+  const int n = (unit->t_hi + p.T - 1) / p.T;
   int32_t* out = p.sel + (int64_t)uid * p.budget;
   if (n <= p.budget) {  // every block
     if (rank == 0)
@@ -171,56 +317,60 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
   }
   const int g = p.g, lo = p.first, hi = n - p.last;  // scored blocks [lo, hi)
   // ---- the query heads in whole numbers, one warp per head ----
-  if (warp < 8) {
+#pragma unroll
+  for (int hq = warp; hq < 8; hq += kSelWarps) {
     float x[D / 32], mx = 0.f;
-    const int64_t q0 = ((int64_t)un.qo_row * p.Hq + (int64_t)h * g + warp) * D;
+    const int64_t q0 = ((int64_t)qo_row * p.Hq + (int64_t)h * g + hq) * D;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      x[i] = warp < g ? load_in(p.q, q0 + lane + 32 * i, p.q_dtype) : 0.f;
+      x[i] = hq < g ? load_in(p.q, q0 + lane + 32 * i, p.q_dtype) : 0.f;
       if (!isfinite(x[i])) x[i] = 0.f;
       mx = fmaxf(mx, fabsf(x[i]));
     }
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    // (non-negative floats order like their bits)
+    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
     const float tau = __fdiv_rn(mx, 127.0f);
     const float inv = tau > 0.f ? __fdiv_rn(1.0f, tau) : 0.f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const int a = max(-127, min(127, __float2int_rn(__fmul_rn(x[i], inv))));
-      qa[warp][lane + 32 * i] = (int8_t)a;
-      qa[warp][D + lane + 32 * i] = (int8_t)abs(a);
+      qa[hq][lane + 32 * i] = (int8_t)a;
+      qa[hq][D + lane + 32 * i] = (int8_t)abs(a);
     }
-    if (lane == 0) tau_s[warp] = tau;
+    if (lane == 0) tau_s[hq] = tau;
   }
   __syncthreads();
   const int r = lane >> 2, tig = lane & 3;
-  uint4 bq[2 * D / 64];  // column r = query head r
+  constexpr int NC = 2 * D / 64;
+  uint4 bq[NC];  // column r = query head r
 #pragma unroll
-  for (int c = 0; c < 2 * D / 64; ++c) bq[c] = *reinterpret_cast<const uint4*>(&qa[r][64 * c + 16 * tig]);
+  for (int c = 0; c < NC; ++c) bq[c] = *reinterpret_cast<const uint4*>(&qa[r][64 * c + 16 * tig]);
   const float tau0 = tau_s[2 * tig], tau1 = tau_s[2 * tig + 1];
   const bool has0 = 2 * tig < g, has1 = 2 * tig + 1 < g;
   uint32_t* keys = p.scratch ? p.scratch + (int64_t)uid * p.scratch_stride
                              : cluster.map_shared_rank(keys_smem, 0);
-  const int32_t* bt = p.bt + (int64_t)un.si * p.bt_stride;
-  const uint8_t* base = p.pool + ((int64_t)un.layer * p.Hkv + h) * p.page_bytes + p.sum_off;
+  const int32_t* bt = p.bt + (int64_t)si * p.bt_stride;
+  const uint8_t* base = p.pool + ((int64_t)layer * p.Hkv + h) * p.page_bytes + p.sum_off;
   const int64_t blk_stride = (int64_t)p.L * p.Hkv * p.page_bytes;
-  for (int i0 = lo + 16 * (rank * (kSelThreads / 32) + warp); i0 < hi; i0 += 16 * CL * (kSelThreads / 32)) {
+  const int spb_bytes = p.spb * 2 * D;
+#pragma unroll 2
+  for (int i0 = lo + 16 * (rank * kSelWarps + warp); i0 < hi; i0 += 16 * CL * kSelWarps) {
     const int ra = min(i0 + r, hi - 1), rb = min(i0 + r + 8, hi - 1);
-    const uint8_t* pa = base + (int64_t)bt[ra / p.spb] * blk_stride;
-    const uint8_t* pb = base + (int64_t)bt[rb / p.spb] * blk_stride;
+    const uint8_t* pa = base + (int64_t)__ldg(bt + ra / p.spb) * blk_stride;
+    const uint8_t* pb = base + (int64_t)__ldg(bt + rb / p.spb) * blk_stride;
     const uint4* wa = reinterpret_cast<const uint4*>(pa + (ra % p.spb) * 2 * D) + tig;
     const uint4* wb = reinterpret_cast<const uint4*>(pb + (rb % p.spb) * 2 * D) + tig;
-    const float sa = *reinterpret_cast<const float*>(pa + p.spb * 2 * D + 4 * (ra % p.spb));
-    const float sb = *reinterpret_cast<const float*>(pb + p.spb * 2 * D + 4 * (rb % p.spb));
-    uint4 xa[2 * D / 64], xb[2 * D / 64];
+    const float sa = __ldg(reinterpret_cast<const float*>(pa + spb_bytes) + ra % p.spb);
+    const float sb = __ldg(reinterpret_cast<const float*>(pb + spb_bytes) + rb % p.spb);
+    uint4 xa[NC], xb[NC];
 #pragma unroll
-    for (int c = 0; c < 2 * D / 64; ++c) {
-      xa[c] = wa[4 * c];
-      xb[c] = wb[4 * c];
+    for (int c = 0; c < NC; ++c) {
+      xa[c] = __ldg(wa + 4 * c);
+      xb[c] = __ldg(wb + 4 * c);
     }
     int acc[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int c = 0; c < 2 * D / 64; ++c) {
+    for (int c = 0; c < NC; ++c) {
       imma16832(acc, xa[c].x, xb[c].x, xa[c].y, xb[c].y, bq[c].x, bq[c].y);
       imma16832(acc, xa[c].z, xb[c].z, xa[c].w, xb[c].w, bq[c].z, bq[c].w);
     }
@@ -253,56 +403,13 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
     __syncthreads();
   }
   if (!p.scratch) keys = keys_smem;
-  // ---- the largest key K with at least budget keys >= K ----
-  uint32_t K = 0;
-  int buf = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = K | (1u << bit);
-    int c = 0;
-    for (int i = tid; i < n; i += kSelThreads) c += keys[i] >= cand ? 1 : 0;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) cnt_s[buf][warp] = c;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int k = 0; k < kSelThreads / 32; ++k) total += cnt_s[buf][k];
-    if (total >= p.budget) K = cand;
-    buf ^= 1;
-  }
-  int above = 0;
-  {
-    int c = 0;
-    for (int i = tid; i < n; i += kSelThreads) c += keys[i] > K ? 1 : 0;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) cnt_s[buf][warp] = c;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSelThreads / 32; ++k) above += cnt_s[buf][k];
-    buf ^= 1;
-  }
-  const int need = p.budget - above;  // of the keys equal to K, the first ones
-  // ---- picked indices in ascending order ----
-  int gt_before = 0, eq_before = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < n ? keys[i] : 0u;
-    const bool gt = i < n && k > K, eq = i < n && k == K;
-    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) cnt_s[buf][warp] = __popc(mg) | (__popc(me) << 16);
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) before += cnt_s[buf][w];
-      total += cnt_s[buf][w];
-    }
-    const uint32_t below = (1u << lane) - 1u;
-    const int gb = gt_before + (before & 0xffff) + __popc(mg & below);
-    const int eb = eq_before + (before >> 16) + __popc(me & below);
-    if (gt || (eq && eb < need)) out[gb + min(eb, need)] = i;
-    gt_before += total & 0xffff;
-    eq_before += total >> 16;
-    buf ^= 1;
+  const int want = p.budget - p.first - p.last;
+  if (n <= 32 * kRegKeys) {
+    if (warp == 0) pick_in_registers<1>(keys, n, want, out, sm, 0, lane);
+  } else if (n <= kSelThreads * kRegKeys) {
+    pick_in_registers<kSelWarps>(keys, n, want, out, sm, warp, lane);
+  } else {
+    pick_in_memory(keys, n, p.budget, out, sm, tid, warp, lane);
   }
 }
 
@@ -310,9 +417,9 @@ template <int D>
 cudaError_t launch_select_d(const SelectParams& p, int n_units, int64_t max_n, int num_sms, cudaStream_t stream) {
   const int64_t pairs = (int64_t)n_units * p.Hkv;
   // CTAs per (unit, head): enough to have two CTAs per SM, while each still
-  // has 128 blocks (one pass of its 8 warps) to score
+  // has 64 blocks (one pass of its 4 warps) to score
   int cl = 1;
-  while (cl < 8 && pairs * cl < 2 * num_sms && max_n / (2 * cl) >= 128) cl *= 2;
+  while (cl < 8 && pairs * cl < 2 * num_sms && max_n / (2 * cl) >= 64) cl *= 2;
   if (pairs * cl > INT32_MAX) return cudaErrorInvalidValue;
   const size_t smem = p.scratch ? 0 : (size_t)max_n * 4;
   if (smem > 32 * 1024) {
