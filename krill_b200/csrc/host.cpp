@@ -1195,6 +1195,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   ap.qt = qt2 ? 2 : 1;
   ap.split_units = reinterpret_cast<const int32_t*>(slot->d + units_bytes + items_bytes + off_bytes + bt_bytes);
   ap.n_split_units = (int)pl.split_units.size();
+  ap.max_cols = std::min(fold, n_query) * g.g;
   ap.q = q;
   ap.q_dtype = q_dtype;
   ap.out = out;
@@ -3478,6 +3479,7 @@ krill_status_t noalloc_plan(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   ap.hg = g.Hkv;
   ap.bt_stride = (int)bt_stride;
   ap.n_split_units = (int)n_su;
+  ap.max_cols = g.g;
   ap.q = q;
   ap.q_dtype = q_dtype;
   ap.out = out;

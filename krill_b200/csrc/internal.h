@@ -117,6 +117,7 @@ struct AttnParams {
   int bt_stride;
   const int32_t* split_units;  // units with n_split > 1
   int n_split_units;
+  int max_cols;                // most query-tile columns of a unit of the launch (combine grid)
   // Arrival counters of split units, one per partial record ((first_split +
   // i) * Hkv + h, only i = 0 used): the decode piece that arrives last merges
   // the unit's records. Each word is (epoch << 32 | arrivals); a word from

@@ -169,19 +169,16 @@ cudaError_t launch_cc(const AttnParams& p, int grid, cudaStream_t stream) {
     default: break;
   }
   if (e != cudaSuccess || p.n_split_units == 0) return e;
-  attn_combine_kernel<D><<<p.n_split_units * p.Hkv, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return run_combine<D>(p, stream);
 }
 }  // namespace
 
 cudaError_t launch_combine(const Geom& g, const AttnParams& p, cudaStream_t stream) {
   if (p.n_split_units == 0) return cudaSuccess;
-  const unsigned blocks = (unsigned)p.n_split_units * p.Hkv;
-  if (g.D == 64) attn_combine_kernel<64><<<blocks, 128, 0, stream>>>(p);
-  else if (g.D == 128) attn_combine_kernel<128><<<blocks, 128, 0, stream>>>(p);
-  else if (g.D == 256) attn_combine_kernel<256><<<blocks, 128, 0, stream>>>(p);
-  else return cudaErrorInvalidValue;
-  return cudaGetLastError();
+  if (g.D == 64) return run_combine<64>(p, stream);
+  if (g.D == 128) return run_combine<128>(p, stream);
+  if (g.D == 256) return run_combine<256>(p, stream);
+  return cudaErrorInvalidValue;
 }
 
 

@@ -474,11 +474,11 @@ __device__ __forceinline__ void tc_subblock_raw(const uint8_t* __restrict__ sb, 
 // subnormal c * 2^-24 (nibble at bit 0 of a half) or 16 c * 2^-24 (bit 4),
 // which the tensor core multiplies exactly. The powers of two are folded into
 // the query (elements k + 8 of a tile carry 1/16) and into the output rows.
-// What is rounded: p s to f16 (as p is on the int8 path); the query is exact
-// (normalised by a power of two per head). To keep that rounding error at the
-// size of the values and not of the codes' offset, z is split as
-// (z + 7.5 s) - 7.5 s, and the second part uses the rounded p s (their sum
-// comes from one more MMA against ones). Each sub-block's P.V starts from zero
+// What is rounded: p to f16 (as on the int8 path), p s to f16 and z + 7.5 s to
+// f16; the query is exact (normalised by a power of two per head). To keep the
+// rounding error of p s at the size of the values and not of the codes'
+// offset, z is split as (z + 7.5 s) - 7.5 s, and the second part uses the
+// rounded p s (their sum comes from one more MMA against a constant). Each sub-block's P.V starts from zero
 // accumulators and joins the running output by one f32 fma per element, which
 // is also its rescale: the truncation of the tensor core's accumulation, a
 // bias on sums of non-negative codes, does not build up over a long sequence.
@@ -487,14 +487,16 @@ __device__ __forceinline__ void tc_subblock_raw(const uint8_t* __restrict__ sb, 
 template <int NG>
 struct Q4State {
   float cs[2];      // softmax scale * log2(e) * 2^24 / normalisation, per column
-  float qs[2][NG];  // sum of the normalised query over a group, * 2^-24
-  float zs[2][NG];  // sum of p (z + 7.5 s) over this lane's tokens
-  float sp[2][NG];  // sum of the rounded p s
+  float zs[2][NG];  // sum of p (z + 7.5 s) over this lane's tokens, less an eighth of 7.5 sum (p s)
+  uint32_t zb[2];   // the group sums of the query, as the B operand of the zeros' MMA (see set_q4)
 };
-struct Q4None {};
+__device__ __forceinline__ float2 q4_floats(uint32_t w, int q_dtype) {
+  return q_dtype == 1 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(u2h(w));
+}
 
 // st.qf and x from fetched words: q * f in f16 with f a power of two that puts
-// the head's largest element in [2^12, 2^13).
+// the head's largest element in [2^14, 2^15). A negative softmax scale enters
+// by its sign here, so that the scores' scale is positive.
 template <int D, int NG>
 __device__ __forceinline__ void set_q4(TCState<D>& st, Q4State<NG>& x, const QRaw<D>& qr, int q_dtype,
                                        float scale_log2, int lane) {
@@ -506,15 +508,14 @@ __device__ __forceinline__ void set_q4(TCState<D>& st, Q4State<NG>& x, const QRa
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = q_dtype == 1 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
-                                    : __half22float2(u2h(w[i]));
+      const float2 v = q4_floats(w[i], q_dtype);
       mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
     }
   }
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const int fe = min(max(266 - (int)(__float_as_uint(mx) >> 23), 1), 253);  // biased exponent of f
-  const float f = __uint_as_float((uint32_t)fe << 23);
+  const int fe = min(max(268 - (int)(__float_as_uint(mx) >> 23), 1), 253);  // biased exponent of f
+  const float f = copysignf(__uint_as_float((uint32_t)fe << 23), scale_log2);
   float sum[NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) sum[g] = 0.f;
@@ -524,100 +525,128 @@ __device__ __forceinline__ void set_q4(TCState<D>& st, Q4State<NG>& x, const QRa
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = q_dtype == 1 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
-                                    : __half22float2(u2h(w[i]));
+      const float2 v = q4_floats(w[i], q_dtype);
       const float lo = v.x * f, hi = v.y * f;
       sum[hh * NG / (D / 64)] += lo + hi;
       st.qf[hh][i] = (i & 1) ? f2h2(lo * 0.0625f, hi * 0.0625f) : f2h2(lo, hi);
     }
   }
-  const float cs = scale_log2 * __uint_as_float((uint32_t)(254 - fe) << 23) * 16777216.f;
+  // (not below 1e-37, so that a masked score of -inf stays one for a scale of 0)
+  const float cs = fmaxf(fabsf(scale_log2) * __uint_as_float((uint32_t)(254 - fe) << 23) * 16777216.f, 1e-37f);
 #pragma unroll
   for (int c = 0; c < 2; ++c) x.cs[c] = __shfl_sync(0xffffffffu, cs, (2 * tig + c) * 4);
+  // The zeros' term sum_g z_tg Q_g, Q_g = 2^-24 sum of the normalised query
+  // over group g, is one MMA per token tile: lane tig = g of a token row holds
+  // (z, z) at k = 2g, 2g + 1 and again at k + 8, and of a column the f16 parts
+  // of Q_g there, high, middle and low. What they leave out is below 2^-25.
+  float mine = 0.f;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     float t = sum[g] + __shfl_xor_sync(0xffffffffu, sum[g], 1);
     t += __shfl_xor_sync(0xffffffffu, t, 2);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      x.qs[c][g] = __shfl_sync(0xffffffffu, t, (2 * tig + c) * 4) * 5.9604644775390625e-08f;  // 2^-24
-      x.zs[c][g] = 0.f;
-      x.sp[c][g] = 0.f;
-    }
+    if (tig == g) mine = t * 5.9604644775390625e-08f;  // 2^-24
+    x.zs[0][g] = x.zs[1][g] = 0.f;
   }
+  const __half h0 = __float2half_rn(mine);
+  const float r0 = mine - __half2float(h0);
+  const __half h1 = __float2half_rn(r0), h2 = __float2half_rn(r0 - __half2float(h1));
+  x.zb[0] = h2u(__halves2half2(h0, h1));
+  x.zb[1] = h2u(__halves2half2(h2, __ushort_as_half(0)));
 }
 
-__device__ __forceinline__ float2 q4_pair(const uint4& w, int u) {
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  return __half22float2(u2h(v[u]));
+__device__ __forceinline__ uint32_t q4_word(const uint4& w, int u) {
+  return u == 0 ? w.x : u == 1 ? w.y : u == 2 ? w.z : w.w;
 }
+__device__ __forceinline__ float2 q4_pair(const uint4& w, int u) { return __half22float2(u2h(q4_word(w, u))); }
 
-// tc_subblock for 4-bit pools (same arguments; row r of token tile u is token
-// 16u + r, rows r + 8 the tokens 8 further).
-template <int D, int NG, int QT>
-__device__ __forceinline__ void tc_subblock4(const uint8_t* __restrict__ sb, TCState<D> (&st)[QT],
-                                             Q4State<NG> (&x)[QT], int lane, float bias, bool boundary,
-                                             int pos0, int t_lo, int t_hi, const int (&th)[QT][2]) {
+// tc_subblock for 4-bit pools in two parts (same arguments; row r of token
+// tile u is token 16u + r, rows r + 8 the tokens 8 further): the K half gives
+// the scores s and, after the online softmax, p * 2^bias in their place, the
+// f16 pairs ph and the rescale al of what came before; the V half adds P.V.
+// ILV token tiles (K) or row tiles (V) advance together, so that consecutive
+// MMAs are independent.
+template <int D, int NG, int QT, int ILV>
+__device__ __forceinline__ void q4_scores(const uint8_t* __restrict__ sb, TCState<D> (&st)[QT],
+                                          Q4State<NG> (&x)[QT], int lane, bool boundary, int pos0, int t_lo,
+                                          const int (&th)[QT][2], float (&s)[QT][4][4]) {
   using SG = SubGeom<D, NG, kFmtInt4>;
   constexpr int NHH = D / 64, HPG = NHH / NG, NU = SG::NU;
   static_assert(NU == 4 && NHH % NG == 0, "four token tiles per sub-block, groups of whole 64-element runs");
-  const int r = lane >> 2;
-  const uint8_t* meta = sb + SG::META + r * 16;  // + (a * NG + group) * 128
+  const int r = lane >> 2, tig = lane & 3;
+  const uint8_t* meta = sb + SG::META4 + r * 16;  // scales, + (NG + group) * 128 zeros
 
-  // ---- K phase ----
-  float s[QT][NU][4];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const uint4 ksw = *reinterpret_cast<const uint4*>(meta + g * 128);
-    const uint4 kzw = *reinterpret_cast<const uint4*>(meta + (NG + g) * 128);
+  // s = sum_g z Q_g, then + s_g (q . c)_g
+  {
+    const uint4 kzw = *reinterpret_cast<const uint4*>(meta + (NG + min(tig, NG - 1)) * 128);
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      float acc[QT][4];
-#pragma unroll
-      for (int q = 0; q < QT; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
-#pragma unroll
-      for (int hg = 0; hg < HPG; ++hg) {
-        const int hh = g * HPG + hg;
-        const uint4 w4 = *reinterpret_cast<const uint4*>(sb + ((u * NHH + hh) * 32 + lane) * 16);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t v = w[k] >> 8;
-          const uint32_t a0 = w[k] & 0x000f000fu, a2 = w[k] & 0x00f000f0u;
-          const uint32_t a1 = v & 0x000f000fu, a3 = v & 0x00f000f0u;
-#pragma unroll
-          for (int q = 0; q < QT; ++q)
-            mma16816(acc[q], a0, a1, a2, a3, st[q].qf[hh][2 * k], st[q].qf[hh][2 * k + 1]);
-        }
-      }
-      const float2 ks = q4_pair(ksw, u), kz = q4_pair(kzw, u);
+      const uint32_t za = __byte_perm(q4_word(kzw, u), 0, 0x1010), zb = __byte_perm(q4_word(kzw, u), 0, 0x3232);
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float part = fmaf(acc[q][c], c < 2 ? ks.x : ks.y, (c < 2 ? kz.x : kz.y) * x[q].qs[c & 1][g]);
-          s[q][u][c] = g == 0 ? part : s[q][u][c] + part;
-        }
+        s[q][u][0] = s[q][u][1] = s[q][u][2] = s[q][u][3] = 0.f;
+        mma16816(s[q][u], za, zb, za, zb, x[q].zb[0], x[q].zb[1]);
       }
     }
   }
 #pragma unroll
-  for (int q = 0; q < QT; ++q)
+  for (int g = 0; g < NG; ++g) {
+    const uint4 ksw = *reinterpret_cast<const uint4*>(meta + g * 128);
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
+    for (int u0 = 0; u0 < NU; u0 += ILV) {
+      float acc[QT][ILV][4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[q][u][c] *= x[q].cs[c & 1];
-      if (boundary) {
+      for (int q = 0; q < QT; ++q)
+#pragma unroll
+        for (int i = 0; i < ILV; ++i) acc[q][i][0] = acc[q][i][1] = acc[q][i][2] = acc[q][i][3] = 0.f;
+#pragma unroll
+      for (int hg = 0; hg < HPG; ++hg) {
+        const int hh = g * HPG + hg;
+        uint4 w[ILV];
+#pragma unroll
+        for (int i = 0; i < ILV; ++i)
+          w[i] = *reinterpret_cast<const uint4*>(sb + (((u0 + i) * NHH + hh) * 32 + lane) * 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < ILV; ++i) {
+            const uint32_t c = q4_word(w[i], k), v = c >> 8;
+            const uint32_t a0 = c & 0x000f000fu, a2 = c & 0x00f000f0u;
+            const uint32_t a1 = v & 0x000f000fu, a3 = v & 0x00f000f0u;
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+              mma16816(acc[q][i], a0, a1, a2, a3, st[q].qf[hh][2 * k], st[q].qf[hh][2 * k + 1]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < ILV; ++i) {
+        const float2 ks = q4_pair(ksw, u0 + i);
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            s[q][u0 + i][c] = fmaf(acc[q][i][c], c < 2 ? ks.x : ks.y, s[q][u0 + i][c]);
+      }
+    }
+  }
+  if (boundary) {
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
         const int pa = pos0 + 16 * u + r, pb = pa + 8;
         if (pa < t_lo || pa >= th[q][0]) s[q][u][0] = -INFINITY;
         if (pa < t_lo || pa >= th[q][1]) s[q][u][1] = -INFINITY;
         if (pb < t_lo || pb >= th[q][0]) s[q][u][2] = -INFINITY;
         if (pb < t_lo || pb >= th[q][1]) s[q][u][3] = -INFINITY;
       }
-    }
+  }
 
-  // ---- online softmax; s becomes p * 2^bias ----
-  float al[QT][2];
+}
+
+template <int D, int NG, int QT>
+__device__ __forceinline__ void q4_softmax(TCState<D> (&st)[QT], const Q4State<NG> (&x)[QT], float bias,
+                                           float (&s)[QT][4][4], uint32_t (&ph)[QT][4][2], float (&al)[QT][2]) {
+  constexpr int NU = 4;
 #pragma unroll
   for (int q = 0; q < QT; ++q) {
     float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -631,7 +660,7 @@ __device__ __forceinline__ void tc_subblock4(const uint8_t* __restrict__ sb, TCS
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
     }
-    const float mn0 = fmaxf(st[q].m[0], mx0), mn1 = fmaxf(st[q].m[1], mx1);
+    const float mn0 = fmaxf(st[q].m[0], mx0 * x[q].cs[0]), mn1 = fmaxf(st[q].m[1], mx1 * x[q].cs[1]);
     const float b0 = (mn0 == -INFINITY) ? 0.f : mn0;
     const float b1 = (mn1 == -INFINITY) ? 0.f : mn1;
     al[q][0] = ex2_ftz(st[q].m[0] - b0);
@@ -642,72 +671,96 @@ __device__ __forceinline__ void tc_subblock4(const uint8_t* __restrict__ sb, TCS
     float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      s[q][u][0] = ex2_ftz(s[q][u][0] + e0);
-      s[q][u][1] = ex2_ftz(s[q][u][1] + e1);
-      s[q][u][2] = ex2_ftz(s[q][u][2] + e0);
-      s[q][u][3] = ex2_ftz(s[q][u][3] + e1);
+      s[q][u][0] = ex2_ftz(fmaf(s[q][u][0], x[q].cs[0], e0));
+      s[q][u][1] = ex2_ftz(fmaf(s[q][u][1], x[q].cs[1], e1));
+      s[q][u][2] = ex2_ftz(fmaf(s[q][u][2], x[q].cs[0], e0));
+      s[q][u][3] = ex2_ftz(fmaf(s[q][u][3], x[q].cs[1], e1));
       ps0 += s[q][u][0] + s[q][u][2];
       ps1 += s[q][u][1] + s[q][u][3];
+      ph[q][u][0] = f2h2(s[q][u][0], s[q][u][1]);
+      ph[q][u][1] = f2h2(s[q][u][2], s[q][u][3]);
     }
     st[q].l[0] = st[q].l[0] * al[q][0] + ps0;
     st[q].l[1] = st[q].l[1] * al[q][1] + ps1;
   }
 
-  // ---- V phase ----
+}
+
+// The weights times the V scales as B operands, per group, and the zeros' part
+// of the output; s and ph are not needed after it.
+template <int D, int NG, int QT>
+__device__ __forceinline__ void q4_weights(const uint8_t* __restrict__ vb, Q4State<NG> (&x)[QT], int lane,
+                                           bool boundary, int pos0, int t_lo, int t_hi, const float (&s)[QT][4][4],
+                                           const uint32_t (&ph)[QT][4][2], const float (&al)[QT][2],
+                                           uint32_t (&pb)[QT][NG][4][2]) {
+  constexpr int NU = 4;
+  const int r = lane >> 2;
+  const uint8_t* meta = vb + SubGeom<D, NG, kFmtInt4>::META4 + r * 16;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    uint4 vsw = *reinterpret_cast<const uint4*>(meta + (2 * NG + g) * 128);
-    uint4 vzw = *reinterpret_cast<const uint4*>(meta + (3 * NG + g) * 128);
+    uint4 vsw = *reinterpret_cast<const uint4*>(meta + g * 128);
+    uint4 vzw = *reinterpret_cast<const uint4*>(meta + (NG + g) * 128);
     if (boundary) {  // a token outside the range may hold any scale: it counts as zero
       uint32_t mk[4];
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int pa = pos0 + 16 * u + r, pb = pa + 8;
-        mk[u] = ((pa >= t_lo && pa < t_hi) ? 0x0000ffffu : 0u) | ((pb >= t_lo && pb < t_hi) ? 0xffff0000u : 0u);
+        const int pa = pos0 + 16 * u + r, pc = pa + 8;
+        mk[u] = ((pa >= t_lo && pa < t_hi) ? 0x0000ffffu : 0u) | ((pc >= t_lo && pc < t_hi) ? 0xffff0000u : 0u);
       }
       vsw = make_uint4(vsw.x & mk[0], vsw.y & mk[1], vsw.z & mk[2], vsw.w & mk[3]);
       vzw = make_uint4(vzw.x & mk[0], vzw.y & mk[1], vzw.z & mk[2], vzw.w & mk[3]);
     }
-    uint32_t pb[QT][NU][2];
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
       float zs0 = 0.f, zs1 = 0.f, one[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const float2 vs = q4_pair(vsw, u), vz = q4_pair(vzw, u);
-        const float za = fmaf(7.5f, vs.x, vz.x), zb = fmaf(7.5f, vs.y, vz.y);
-        zs0 = fmaf(s[q][u][0], za, fmaf(s[q][u][2], zb, zs0));
-        zs1 = fmaf(s[q][u][1], za, fmaf(s[q][u][3], zb, zs1));
-        pb[q][u][0] = movm_trans(f2h2(s[q][u][0] * vs.x, s[q][u][1] * vs.x));
-        pb[q][u][1] = movm_trans(f2h2(s[q][u][2] * vs.y, s[q][u][3] * vs.y));
-        mma16816(one, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[q][u][0], pb[q][u][1]);
+        const uint32_t vs = q4_word(vsw, u);
+        const float2 z = __half22float2(__hfma2(u2h(0x47804780u), u2h(vs), u2h(q4_word(vzw, u))));  // z + 7.5 s
+        zs0 = fmaf(s[q][u][0], z.x, fmaf(s[q][u][2], z.y, zs0));
+        zs1 = fmaf(s[q][u][1], z.x, fmaf(s[q][u][3], z.y, zs1));
+        pb[q][g][u][0] = movm_trans(h2u(__hmul2(u2h(ph[q][u][0]), u2h(__byte_perm(vs, 0, 0x1010)))));
+        pb[q][g][u][1] = movm_trans(h2u(__hmul2(u2h(ph[q][u][1]), u2h(__byte_perm(vs, 0, 0x3232)))));
+        mma16816(one, 0x3b803b80u, 0x3b803b80u, 0x3b803b80u, 0x3b803b80u, pb[q][g][u][0], pb[q][g][u][1]);  // 7.5 / 8
       }
-      x[q].zs[0][g] = fmaf(x[q].zs[0][g], al[q][0], zs0);
-      x[q].zs[1][g] = fmaf(x[q].zs[1][g], al[q][1], zs1);
-      x[q].sp[0][g] = fmaf(x[q].sp[0][g], al[q][0], one[0]);
-      x[q].sp[1][g] = fmaf(x[q].sp[1][g], al[q][1], one[1]);
+      x[q].zs[0][g] = fmaf(x[q].zs[0][g], al[q][0], zs0 - one[0]);
+      x[q].zs[1][g] = fmaf(x[q].zs[1][g], al[q][1], zs1 - one[1]);
+    }
+  }
+}
+
+template <int D, int NG, int QT, int ILV>
+__device__ __forceinline__ void q4_output(const uint8_t* __restrict__ vb, TCState<D> (&st)[QT], int lane,
+                                          const uint32_t (&pb)[QT][NG][4][2], const float (&al)[QT][2]) {
+  constexpr int NU = 4, MG = D / 16 / NG;
+#pragma unroll
+  for (int mt0 = 0; mt0 < D / 16; mt0 += ILV) {
+    const int g = mt0 / MG;
+    uint4 w[ILV];
+    float acc[QT][ILV][4];
+#pragma unroll
+    for (int i = 0; i < ILV; ++i) {
+      w[i] = *reinterpret_cast<const uint4*>(vb + ((mt0 + i) * 32 + lane) * 16);
+#pragma unroll
+      for (int q = 0; q < QT; ++q) acc[q][i][0] = acc[q][i][1] = acc[q][i][2] = acc[q][i][3] = 0.f;
     }
 #pragma unroll
-    for (int mi = 0; mi < SG::G / 16; ++mi) {
-      const int mt = g * (SG::G / 16) + mi;
-      const uint4 w4 = *reinterpret_cast<const uint4*>(sb + SG::VOFF + (mt * 32 + lane) * 16);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      float acc[QT][4];
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-      for (int q = 0; q < QT; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const uint32_t v = w[u] >> 8;
-        const uint32_t a0 = w[u] & 0x000f000fu, a1 = w[u] & 0x00f000f0u;
+      for (int i = 0; i < ILV; ++i) {
+        const uint32_t c = q4_word(w[i], u), v = c >> 8;
+        const uint32_t a0 = c & 0x000f000fu, a1 = c & 0x00f000f0u;
         const uint32_t a2 = v & 0x000f000fu, a3 = v & 0x00f000f0u;
 #pragma unroll
-        for (int q = 0; q < QT; ++q) mma16816(acc[q], a0, a1, a2, a3, pb[q][u][0], pb[q][u][1]);
+        for (int q = 0; q < QT; ++q) mma16816(acc[q][i], a0, a1, a2, a3, pb[q][g][u][0], pb[q][g][u][1]);
       }
 #pragma unroll
-      for (int q = 0; q < QT; ++q)
+    for (int q = 0; q < QT; ++q)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) st[q].o[mt][c] = fmaf(st[q].o[mt][c], al[q][c & 1], acc[q][c]);
-    }
+      for (int i = 0; i < ILV; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          st[q].o[mt0 + i][c] = fmaf(st[q].o[mt0 + i][c], al[q][c & 1], acc[q][i][c]);
   }
 }
 
@@ -720,10 +773,9 @@ __device__ __forceinline__ void finalize4(TCState<D>& st, const Q4State<NG>& x, 
     float z[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float t = x.zs[c][g];
+      z[c] = x.zs[c][g];
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) t += __shfl_xor_sync(0xffffffffu, t, off);
-      z[c] = fmaf(-7.5f, x.sp[c][g], t);
+      for (int off = 4; off < 32; off <<= 1) z[c] += __shfl_xor_sync(0xffffffffu, z[c], off);
     }
     constexpr int MG = D / 16 / NG;
 #pragma unroll
@@ -749,12 +801,13 @@ struct AttnSmem {
   static constexpr int TOTAL = MISC_OFF + 16;
 };
 
-// Number of 64-token stages that fit next to the rest of the shared memory.
+// Number of stages that fit next to the rest of the shared memory.
 template <int D, int NG, int NCW, int R, int FMT = kFmtInt8>
 constexpr int stages_for() {
   constexpr int fixed = AttnSmem<D, NG, NCW, R, 0, FMT>::TOTAL;
-  constexpr int n = (232448 - fixed - 2 * 16 * 8) / SubGeom<D, NG, FMT>::SB;
-  return n > 16 ? 16 : n;
+  constexpr int most = FMT == kFmtInt4 ? 24 : 16;
+  constexpr int n = (232448 - fixed - 2 * 8 * most - (FMT == kFmtInt4 ? 4 * most : 0)) / AttnSmem<D, NG, NCW, R, 0, FMT>::SB;
+  return n > most ? most : n;
 }
 
 // Merge a split unit's n_split partial records for kv head h into the output,
@@ -949,49 +1002,72 @@ __device__ __forceinline__ void finish_head(const AttnParams& p, TCState<D>& st,
   if (p.split_ctr != nullptr && arrive_split(p, un, h, lane)) merge_split<D>(p, un, h, lane);
 }
 
-// Merge the partial records of split units: one CTA per (split unit, kv head).
+// Merge the partial records of split units: one warp per (split unit, kv head,
+// column of the query tile). Lane i of the warp holds the max and normalizer of
+// record i (32 at a time), the lanes together one row of D outputs, and the
+// records' rows are summed in record order, eight of them in flight. Reads
+// bound it: one CTA per (unit, kv head) whose 128 threads walked all the
+// columns took 106 us for 12 x 2 x 4 (unit, head) pairs of 32 records at
+// head_dim 128 (12.8 MB).
+constexpr int kCombineWarps = 4;
 template <int D>
-__global__ void __launch_bounds__(128) attn_combine_kernel(AttnParams p) {
-  const int Hkv = p.Hkv, g = p.g;
-  const int u = p.split_units[blockIdx.x / Hkv];
-  const int h = blockIdx.x % Hkv;
-  const AttnUnit un = p.units[u];
+__global__ void __launch_bounds__(32 * kCombineWarps) attn_combine_kernel(AttnParams p) {
+  constexpr int V = D < 128 ? 2 : 4, EPT = D / (32 * V);  // EPT vectors of V floats per lane
+  using Vec = typename std::conditional<V == 4, float4, float2>::type;
+  const int Hkv = p.Hkv, g = p.g, lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
+  const int hq = (int)(w % p.max_cols), h = (int)(w / p.max_cols % Hkv);
+  const int64_t ui = w / p.max_cols / Hkv;
+  if (ui >= p.n_split_units) return;
+  const AttnUnit un = p.units[p.split_units[ui]];
+  if (hq >= unit_cols(un, g)) return;
   const float* base = p.partials + ((int64_t)un.first_split * Hkv + h) * partial_floats(D);
   const int64_t stride = (int64_t)Hkv * partial_floats(D);
-  // (loops unrolled so that several records' loads are in flight; the sums
-  // keep record order)
-  const int cols = unit_cols(un, g);
-  const int64_t row_elems = (int64_t)p.Hq * D;
-  __shared__ float sm[8], sinv[8];
-  if (threadIdx.x < cols) {
-    const int hq = threadIdx.x;
-    float M = -INFINITY;
+  const int n = un.n_split;
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, base[i * stride + hq]);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float Ls = 0.f, Os[EPT][V];
+#pragma unroll
+  for (int e = 0; e < EPT; ++e)
+#pragma unroll
+    for (int c = 0; c < V; ++c) Os[e][c] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane, m = min(32, n - i0);
+    const float mi = i < n ? base[i * stride + hq] : -INFINITY;
+    const float li = i < n ? base[i * stride + 8 + hq] : 0.f;
+    const float wi = mi == -INFINITY ? 0.f : exp2f(mi - M);
+    const float* o = base + i0 * stride + 16 + hq * D + lane * V;
 #pragma unroll 8
-    for (int i = 0; i < un.n_split; ++i) M = fmaxf(M, base[i * stride + hq]);
-    float Ls = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < un.n_split; ++i) {
-      const float mi = base[i * stride + hq];
-      const float li = base[i * stride + 8 + hq];
-      Ls += (mi == -INFINITY) ? 0.f : li * exp2f(mi - M);
+    for (int k = 0; k < m; ++k) {
+      Vec x[EPT];
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) x[e] = *reinterpret_cast<const Vec*>(o + k * stride + e * 32 * V);
+      const float mk = __shfl_sync(0xffffffffu, mi, k);
+      const float lk = __shfl_sync(0xffffffffu, li, k), wk = __shfl_sync(0xffffffffu, wi, k);
+      Ls += (mk == -INFINITY) ? 0.f : lk * wk;
+#pragma unroll
+      for (int e = 0; e < EPT; ++e)
+#pragma unroll
+        for (int c = 0; c < V; ++c) {  // (an empty record's O may be anything)
+          const float oi = reinterpret_cast<const float*>(&x[e])[c];
+          Os[e][c] = (mk != -INFINITY) ? Os[e][c] + oi * wk : Os[e][c];
+        }
     }
-    sm[hq] = M;
-    sinv[hq] = 1.f / Ls;
   }
-  __syncthreads();
-  const int64_t orow = ((int64_t)un.qo_row * p.Hq + (int64_t)h * g) * D;
-  for (int idx = threadIdx.x; idx < cols * D; idx += blockDim.x) {
-    const int hq = idx / D, d = idx - hq * D;
-    const float M = sm[hq];
-    float Os = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < un.n_split; ++i) {
-      const float mi = base[i * stride + hq];
-      const float oi = base[i * stride + 16 + hq * D + d];
-      Os = (mi != -INFINITY) ? Os + oi * exp2f(mi - M) : Os;
-    }
-    store_out(p.out, p.out_dtype, orow + col_off(hq, g, row_elems, D) + d, Os * sinv[hq]);
-  }
+  const float inv = 1.f / Ls;
+  const int64_t orow = ((int64_t)un.qo_row * p.Hq + (int64_t)h * g) * D + col_off(hq, g, (int64_t)p.Hq * D, D);
+#pragma unroll
+  for (int e = 0; e < EPT; ++e)
+#pragma unroll
+    for (int c = 0; c < V; ++c) store_out(p.out, p.out_dtype, orow + (e * 32 + lane) * V + c, Os[e][c] * inv);
+}
+template <int D>
+cudaError_t run_combine(const AttnParams& p, cudaStream_t stream) {
+  const int64_t warps = (int64_t)p.n_split_units * p.Hkv * p.max_cols;
+  attn_combine_kernel<D><<<(unsigned)((warps + kCombineWarps - 1) / kCombineWarps), 32 * kCombineWarps, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 // Work split inside a CTA: an item covers hg kv heads; HPR = NCW / R of them
@@ -1007,6 +1083,53 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(AttnParams p) {
 // consumer without spills.)
 constexpr int kProducerRegs = 56;
 constexpr int kConsumerRegs = 224;
+
+// Merges the R warps of one head through a lane-major buffer; warp rr = 0 of
+// them ends with the merged state.
+template <int D, int NCW, int R, typename SM>
+__device__ __forceinline__ void merge_warps(TCState<D>& st, float& l0, float& l1, uint8_t* smem, int hr, int rr,
+                                            int lane) {
+  if constexpr (R > 1) {
+    float* cb = reinterpret_cast<float*>(smem + SM::CB_OFF);
+    const int nbar = 1 + hr;
+    asm volatile("bar.sync %0, %1;" ::"r"(nbar), "r"(R * 32) : "memory");  // buffer free
+    if (rr != 0) {
+      float* mine = cb + (size_t)(hr * (R - 1) + rr - 1) * SM::NV * 32;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mine[(mt * 4 + c) * 32 + lane] = st.o[mt][c];
+      mine[(D / 4 + 0) * 32 + lane] = st.m[0];
+      mine[(D / 4 + 1) * 32 + lane] = st.m[1];
+      mine[(D / 4 + 2) * 32 + lane] = l0;
+      mine[(D / 4 + 3) * 32 + lane] = l1;
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(nbar), "r"(R * 32) : "memory");
+    if (rr == 0) {
+#pragma unroll(R <= 4 ? R : 1)
+      for (int w = 1; w < R; ++w) {
+        const float* o = cb + (size_t)(hr * (R - 1) + w - 1) * SM::NV * 32;
+        const float m0 = o[(D / 4 + 0) * 32 + lane], m1 = o[(D / 4 + 1) * 32 + lane];
+        const float M0 = fmaxf(st.m[0], m0), M1 = fmaxf(st.m[1], m1);
+        const float a0 = (st.m[0] == -INFINITY) ? 0.f : exp2f(st.m[0] - M0);
+        const float a1 = (st.m[1] == -INFINITY) ? 0.f : exp2f(st.m[1] - M1);
+        const float b0 = (m0 == -INFINITY) ? 0.f : exp2f(m0 - M0);
+        const float b1 = (m1 == -INFINITY) ? 0.f : exp2f(m1 - M1);
+        l0 = l0 * a0 + o[(D / 4 + 2) * 32 + lane] * b0;
+        l1 = l1 * a1 + o[(D / 4 + 3) * 32 + lane] * b1;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) {
+          st.o[mt][0] = st.o[mt][0] * a0 + o[(mt * 4 + 0) * 32 + lane] * b0;
+          st.o[mt][1] = st.o[mt][1] * a1 + o[(mt * 4 + 1) * 32 + lane] * b1;
+          st.o[mt][2] = st.o[mt][2] * a0 + o[(mt * 4 + 2) * 32 + lane] * b0;
+          st.o[mt][3] = st.o[mt][3] * a1 + o[(mt * 4 + 3) * 32 + lane] * b1;
+        }
+        st.m[0] = M0;
+        st.m[1] = M1;
+      }
+    }
+  }
+}
 
 // Consumer warps of attn_tc_kernel. FAST selects the one-fma dequantization,
 // exact only while every scale in the pool is below 64 in magnitude; the
@@ -1027,14 +1150,11 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
   using SM = AttnSmem<D, NG, NCW, R, NSTAGE, FMT>;
   constexpr int SB = SM::SB;
   constexpr int HPR = NCW / R;
-  static_assert(QT == 1 || (R == 1 && FMT != kFmtBf16), "two query tiles: one warp per head, quantized pool");
+  static_assert(QT == 1 || (R == 1 && FMT == kFmtInt8), "two query tiles: one warp per head, int8");
   static_assert(QT == 1 || !SEL, "picked blocks: one query per sequence");
   const int hr = warp / R, rr = warp % R;
   TCState<D> sts[QT];
   TCState<D>& st = sts[0];
-  typename std::conditional<FMT == kFmtInt4, Q4State<NG>, Q4None>::type x4[QT];
-  // 4-bit pools: exponent bias of the softmax weights (see tc_subblock4)
-  const float bias = FMT == kFmtInt4 && *reinterpret_cast<volatile const int*>(p.large_scale) == 0 ? 8.f : 0.f;
   uint32_t J = 0;
   AttnItem item_next{};
   AttnUnit un_next{};
@@ -1069,8 +1189,7 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
       if constexpr (QT == 2)
         fetch_q<D>(qr, p.q, q_row(un, h), p.g, unit_cols(un, p.g), q_row_elems, lane);
       reset_state(st);
-      if constexpr (FMT == kFmtInt4) set_q4<D, NG>(st, x4[0], qr, p.q_dtype, p.scale_log2, lane);
-      else set_q<D, FMT>(st, qr, p.q_dtype);
+      set_q<D, FMT>(st, qr, p.q_dtype);
       // the shadow unit's queries (second tile), fetched here: items are long
       // (the shadow record is read again at the finish, not kept in registers)
       AttnUnit un2 = un;
@@ -1079,8 +1198,7 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
         QRaw<D> qr2;
         fetch_q<D>(qr2, p.q, q_row(un2, h), p.g, unit_cols(un2, p.g), q_row_elems, lane);
         reset_state(sts[1]);
-        if constexpr (FMT == kFmtInt4) set_q4<D, NG>(sts[1], x4[1], qr2, p.q_dtype, p.scale_log2, lane);
-        else set_q<D, FMT>(sts[1], qr2, p.q_dtype);
+        set_q<D, FMT>(sts[1], qr2, p.q_dtype);
       }
       // prefetch state: 0 nothing yet, 1 next unit requested, 2 next q fetched
       int pf = 0;
@@ -1133,9 +1251,7 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
           boundary = j == min(p.sel_stride, (t_hi + T - 1) / T) - 1 && pos0 + T > t_hi;
         }
         const uint8_t* sbp = stages + (size_t)stage * SB;
-        if constexpr (FMT == kFmtInt4)
-          tc_subblock4<D, NG, QT>(sbp, sts, x4, lane, bias, boundary, pos0, un.t_lo, t_hi, th);
-        else if constexpr (FMT == kFmtBf16)
+        if constexpr (FMT == kFmtBf16)
           tc_subblock_raw<D>(sbp, st, lane, p.scale_log2, boundary, pos0, un.t_lo, un.t_hi);
         else
           tc_subblock<D, NG, FAST, QT>(sbp, sts, lane, p.scale_log2, boundary, pos0, un.t_lo, t_hi, th);
@@ -1146,57 +1262,13 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
       while (pf < 2) prefetch_step();
       J += (uint32_t)n_sb * HPR;
 
-      if constexpr (FMT == kFmtInt4) {
-#pragma unroll
-        for (int q = 0; q < QT; ++q) finalize4<D, NG>(sts[q], x4[q], bias);
-      }
       float l0 = st.l[0], l1 = st.l[1];
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, off);
         l1 += __shfl_xor_sync(0xffffffffu, l1, off);
       }
-      if constexpr (R > 1) {
-        // merge the R warps of this head through a lane-major buffer
-        float* cb = reinterpret_cast<float*>(smem + SM::CB_OFF);
-        const int nbar = 1 + hr;
-        asm volatile("bar.sync %0, %1;" ::"r"(nbar), "r"(R * 32) : "memory");  // buffer free
-        if (rr != 0) {
-          float* mine = cb + (size_t)(hr * (R - 1) + rr - 1) * SM::NV * 32;
-#pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) mine[(mt * 4 + c) * 32 + lane] = st.o[mt][c];
-          mine[(D / 4 + 0) * 32 + lane] = st.m[0];
-          mine[(D / 4 + 1) * 32 + lane] = st.m[1];
-          mine[(D / 4 + 2) * 32 + lane] = l0;
-          mine[(D / 4 + 3) * 32 + lane] = l1;
-        }
-        asm volatile("bar.sync %0, %1;" ::"r"(nbar), "r"(R * 32) : "memory");
-        if (rr == 0) {
-#pragma unroll
-          for (int w = 1; w < R; ++w) {
-            const float* o = cb + (size_t)(hr * (R - 1) + w - 1) * SM::NV * 32;
-            const float m0 = o[(D / 4 + 0) * 32 + lane], m1 = o[(D / 4 + 1) * 32 + lane];
-            const float M0 = fmaxf(st.m[0], m0), M1 = fmaxf(st.m[1], m1);
-            const float a0 = (st.m[0] == -INFINITY) ? 0.f : exp2f(st.m[0] - M0);
-            const float a1 = (st.m[1] == -INFINITY) ? 0.f : exp2f(st.m[1] - M1);
-            const float b0 = (m0 == -INFINITY) ? 0.f : exp2f(m0 - M0);
-            const float b1 = (m1 == -INFINITY) ? 0.f : exp2f(m1 - M1);
-            l0 = l0 * a0 + o[(D / 4 + 2) * 32 + lane] * b0;
-            l1 = l1 * a1 + o[(D / 4 + 3) * 32 + lane] * b1;
-#pragma unroll
-            for (int mt = 0; mt < D / 16; ++mt) {
-              st.o[mt][0] = st.o[mt][0] * a0 + o[(mt * 4 + 0) * 32 + lane] * b0;
-              st.o[mt][1] = st.o[mt][1] * a1 + o[(mt * 4 + 1) * 32 + lane] * b1;
-              st.o[mt][2] = st.o[mt][2] * a0 + o[(mt * 4 + 2) * 32 + lane] * b0;
-              st.o[mt][3] = st.o[mt][3] * a1 + o[(mt * 4 + 3) * 32 + lane] * b1;
-            }
-            st.m[0] = M0;
-            st.m[1] = M1;
-          }
-        }
-      }
+      merge_warps<D, NCW, R, SM>(st, l0, l1, smem, hr, rr, lane);
       if (rr == 0) finish_head<D>(p, st, l0, l1, un, item, h, lane);
       if constexpr (QT == 2) {
         float m0 = sts[1].l[0], m1 = sts[1].l[1];
@@ -1208,6 +1280,162 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
         finish_head<D>(p, sts[1], m0, m1, p.units[item.unit + 1], item, h, lane);
       }
     }
+  }
+}
+
+// Consumer warps for 4-bit pools. Little is kept in registers between items
+// (the producer warp has their records and queries in the caches by then).
+template <int D, int NG, int NCW, int R, int NSTAGE, int QT, bool SEL>
+__device__ __forceinline__ void attn_consume4(const AttnParams& p, uint8_t* smem, uint8_t* stages,
+                                              uint32_t bar_base, volatile int* cta_abort, volatile uint32_t* tags,
+                                              int warp, int lane, int it0, int it1, int rounds) {
+  using SM = AttnSmem<D, NG, NCW, R, NSTAGE, kFmtInt4>;
+  constexpr int SB = SM::SB, HPR = NCW / R, T = kSub4;
+  // token / row tiles advanced together: what the registers allow
+  constexpr int ILV = QT == 2 ? 2 : 4;
+  static_assert(QT == 1 || (R == 1 && !SEL), "two query tiles: one warp per head, whole sequences");
+  const int hr = warp / R, rr = warp % R;
+  // exponent bias of the softmax weights (see Q4State)
+  const float bias = *reinterpret_cast<volatile const int*>(p.large_scale) == 0 ? 8.f : 0.f;
+  const int64_t row_elems = (int64_t)p.Hq * D;
+  uint32_t J = 0;
+  for (int it = it0; it < it1; ++it) {
+    const AttnItem item = p.items[it];
+    const int n_sb = item.sb_end - item.sb_begin;
+    for (int rd = 0; rd < rounds; ++rd) {
+      const int h = item.h0 + rd * HPR + hr;
+      TCState<D> st[QT];
+      Q4State<NG> x[QT];
+      // per-column bounds (AttnUnit::nq) as in attn_consume
+      int th[QT][2], t_lo = 0, t_hi = 0, b_min = INT32_MAX;
+#pragma unroll
+      for (int q = 0; q < QT; ++q) {
+        const AttnUnit un = p.units[item.unit + q];
+        QRaw<D> qr;
+        fetch_q<D>(qr, p.q, ((int64_t)un.qo_row * p.Hq + (int64_t)h * p.g) * D, p.g, unit_cols(un, p.g), row_elems, lane);
+        reset_state(st[q]);
+        set_q4<D, NG>(st[q], x[q], qr, p.q_dtype, p.scale_log2, lane);
+        const int nq1 = un.nq > 1 ? un.nq - 1 : 0;
+        th[q][0] = un.t_hi - (nq1 - min((2 * (lane & 3)) / p.g, nq1));
+        th[q][1] = un.t_hi - (nq1 - min((2 * (lane & 3) + 1) / p.g, nq1));
+        b_min = min(b_min, un.t_hi - nq1);
+        t_hi = max(t_hi, un.t_hi);
+        t_lo = un.t_lo;
+      }
+#pragma unroll 1
+      for (int k = rr; k < n_sb; k += R) {
+        const uint32_t jj = J + (uint32_t)k * HPR + hr;
+        const uint32_t stage = jj % NSTAGE;
+        const int j = item.sb_begin + k;
+        int pos0 = j * T;
+        bool boundary = pos0 < t_lo || pos0 + T > b_min;
+        if constexpr (SEL) {  // only the last picked block, the sequence's last, may be partial
+          pos0 = (t_hi - 1) / T * T;
+          boundary = j == min(p.sel_stride, (t_hi + T - 1) / T) - 1 && pos0 + T > t_hi;
+        }
+        float s[QT][4][4], al[QT][2];
+        uint32_t ph[QT][4][2], pb[QT][NG][4][2];
+        wait_tag(tags + stage, jj, cta_abort, p.err);
+        mbar_wait(bar_base + 8 * stage, (jj / NSTAGE) & 1, cta_abort, p.err);
+        const uint8_t* kb = stages + (size_t)stage * SB;
+        const uint8_t* vb = kb + q4_half(D, NG);
+        q4_scores<D, NG, QT, ILV>(kb, st, x, lane, boundary, pos0, t_lo, th, s);
+        q4_softmax<D, NG, QT>(st, x, bias, s, ph, al);
+        q4_weights<D, NG, QT>(vb, x, lane, boundary, pos0, t_lo, t_hi, s, ph, al, pb);
+        q4_output<D, NG, QT, ILV>(vb, st, lane, pb, al);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_base + 8 * (NSTAGE + stage));
+      }
+      J += (uint32_t)n_sb * HPR;
+#pragma unroll
+      for (int q = 0; q < QT; ++q) {
+        finalize4<D, NG>(st[q], x[q], bias);
+        float l0 = st[q].l[0], l1 = st[q].l[1];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+          l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+        }
+        merge_warps<D, NCW, R, SM>(st[q], l0, l1, smem, hr, rr, lane);
+        if (rr == 0) finish_head<D>(p, st[q], l0, l1, p.units[item.unit + q], item, h, lane);
+      }
+    }
+  }
+}
+
+// Producer of 4-bit pools and of picked blocks: eight lanes issue eight
+// consecutive copies at a time. (A 4-bit sub-block is half an int8 one; issued
+// by one lane, whose wait, tag, arrive and copy follow one another, the copies
+// of the batch of 32 sequences alone took 183 us where their bytes need 139.)
+// Each lane finds the source of its next copy - the picked block's index and
+// the block table entry - before it waits for the stage of the current one.
+template <int D, int NG, int NCW, int R, int NSTAGE, int FMT, bool SEL>
+__device__ __forceinline__ void produce_wide(const AttnParams& p, uint8_t* stages, uint32_t bar_base,
+                                             volatile int* cta_abort, volatile uint32_t* tags, int lane, int it0,
+                                             int it1, int rounds) {
+  using SG = SubGeom<D, NG, FMT>;
+  constexpr int HPR = NCW / R, SB = SG::SB, SPB = SG::SPB, W = 8;
+  static_assert(NSTAGE >= W, "a step's copies must not wait for one another");
+  const int Hkv = p.Hkv;
+  // copy i of round rd of an item: its sub-block i / HPR of head i % HPR
+  auto source = [&](const AttnItem& item, int layer, int si, int rd, int i) {
+    const int h = item.h0 + rd * HPR + i % HPR;
+    int sb = item.sb_begin + i / HPR;
+    if (SEL) sb = __ldg(p.sel + ((int64_t)item.unit * Hkv + h) * p.sel_stride + sb);
+    int bi = sb / SPB;
+    if (p.ring > 0) bi %= p.ring;
+    const int b = __ldg(p.bt + (int64_t)si * p.bt_stride + bi);
+    return p.pool + (((int64_t)b * p.L + layer) * Hkv + h) * p.page_bytes + (int64_t)(sb % SPB) * SB;
+  };
+  if (it0 >= it1) return;
+  AttnItem item = p.items[it0], item_n{};
+  int layer = p.units[item.unit].layer, si = p.units[item.unit].si, layer_n = 0, si_n = 0;
+  const uint8_t* src = nullptr;
+  if (lane < W && lane < (item.sb_end - item.sb_begin) * HPR) src = source(item, layer, si, 0, lane);
+  uint32_t J = 0;
+  for (int it = it0; it < it1; ++it) {
+    if (it + 1 < it1) {
+      item_n = p.items[it + 1];
+      layer_n = p.units[item_n.unit].layer;
+      si_n = p.units[item_n.unit].si;
+      if constexpr (FMT == kFmtInt4) {  // its query rows (adjacent: hg * g of them), for the consumers
+        const AttnUnit* un = p.units + item_n.unit;
+        const char* q0 = static_cast<const char*>(p.q) + ((int64_t)un->qo_row * p.Hq + (int64_t)item_n.h0 * p.g) * D * 2;
+        for (int i = lane * 128; i < p.hg * p.g * D * 2; i += 32 * 128)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(q0 + i));
+      }
+    }
+    const int total = (item.sb_end - item.sb_begin) * HPR;
+    for (int rd = 0; rd < rounds; ++rd) {
+      for (int q = 0; q < total; q += W) {
+        const uint8_t* next = nullptr;
+        if (lane < W) {
+          if (q + W < total) {
+            if (q + W + lane < total) next = source(item, layer, si, rd, q + W + lane);
+          } else if (rd + 1 < rounds) {
+            if (lane < total) next = source(item, layer, si, rd + 1, lane);
+          } else if (it + 1 < it1) {
+            if (lane < (item_n.sb_end - item_n.sb_begin) * HPR) next = source(item_n, layer_n, si_n, 0, lane);
+          }
+        }
+        if (src != nullptr) {
+          const uint32_t Jh = J + (uint32_t)(q + lane);
+          const uint32_t stage = Jh % NSTAGE;
+          if (Jh >= (uint32_t)NSTAGE)
+            mbar_wait(bar_base + 8 * (NSTAGE + stage), ((Jh / NSTAGE) - 1) & 1, cta_abort, p.err);
+          const uint32_t full = bar_base + 8 * stage;
+          tags[stage] = Jh;  // released by the arrive below
+          mbar_expect_tx(full, SB);
+          bulk_g2s(smem_u32(stages + (size_t)stage * SB), src, SB, full);
+        }
+        src = next;
+        __syncwarp();
+      }
+      J += (uint32_t)total;
+    }
+    item = item_n;
+    layer = layer_n;
+    si = si_n;
   }
 }
 
@@ -1273,51 +1501,8 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) attn_tc_kernel(AttnParams p
       if (p.ring > 0) bi %= p.ring;
       return lane < nblk ? p.bt[(int64_t)u.si * p.bt_stride + bi] : 0;
     };
-    if constexpr (SEL) {
-      // Picked blocks: per chunk of 32 list entries, the lanes fetch every
-      // head's sub-block indices and then their block ids; lane 0 issues.
-      uint32_t J = 0;
-      for (int it = it0; it < it1; ++it) {
-        const AttnItem item = p.items[it];
-        const AttnUnit un = p.units[item.unit];
-        const int32_t* bt = p.bt + (int64_t)un.si * p.bt_stride;
-        const int n_sb = item.sb_end - item.sb_begin;
-        for (int rd = 0; rd < rounds; ++rd) {
-          const int h0 = item.h0 + rd * HPR;
-          const uint8_t* layer_base = p.pool + ((int64_t)un.layer * Hkv + h0) * p.page_bytes;
-          const int32_t* sel = p.sel + ((int64_t)item.unit * Hkv + h0) * p.sel_stride + item.sb_begin;
-          for (int c0 = 0; c0 < n_sb; c0 += 32) {
-            int at[HPR];  // block id * SPB + sub-block
-#pragma unroll
-            for (int hr = 0; hr < HPR; ++hr)
-              at[hr] = c0 + lane < n_sb ? sel[(int64_t)hr * p.sel_stride + c0 + lane] : -1;
-#pragma unroll
-            for (int hr = 0; hr < HPR; ++hr)
-              if (at[hr] >= 0) at[hr] = bt[at[hr] / SPB] * SPB + at[hr] % SPB;
-            const int n = min(32, n_sb - c0);
-            for (int k = 0; k < n; ++k) {
-#pragma unroll
-              for (int hr = 0; hr < HPR; ++hr) {
-                const int a = __shfl_sync(0xffffffffu, at[hr], k);
-                if (lane == 0) {
-                  const uint32_t Jh = J + (uint32_t)(c0 + k) * HPR + hr;
-                  const uint32_t stage = Jh % NSTAGE;
-                  if (Jh >= (uint32_t)NSTAGE)
-                    mbar_wait(bar_base + 8 * (NSTAGE + stage), ((Jh / NSTAGE) - 1) & 1, cta_abort, p.err);
-                  const uint32_t full = bar_base + 8 * stage;
-                  tags[stage] = Jh;
-                  mbar_expect_tx(full, SB);
-                  bulk_g2s(smem_u32(stages + (size_t)stage * SB),
-                           layer_base + (int64_t)(a / SPB) * blk_stride + (int64_t)(a % SPB) * SB +
-                               (int64_t)hr * p.page_bytes,
-                           SB, full);
-                }
-              }
-            }
-          }
-          J += (uint32_t)n_sb * HPR;
-        }
-      }
+    if constexpr (SEL || FMT == kFmtInt4) {
+      produce_wide<D, NG, NCW, R, NSTAGE, FMT, SEL>(p, stages, bar_base, cta_abort, tags, lane, it0, it1, rounds);
       return;
     }
     AttnItem item_n{};
@@ -1387,9 +1572,12 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) attn_tc_kernel(AttnParams p
 
   // ---------------- consumers ----------------
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
-  if (FMT == kFmtInt8 && *reinterpret_cast<volatile const int*>(p.large_scale) != 0)
-    attn_consume<D, NG, NCW, R, NSTAGE, FMT, FMT != kFmtInt8, QT, SEL>(p, smem, stages, bar_base, cta_abort, tags,
-                                                                    warp, lane, it0, it1, rounds);
+  if constexpr (FMT == kFmtInt4)
+    attn_consume4<D, NG, NCW, R, NSTAGE, QT, SEL>(p, smem, stages, bar_base, cta_abort, tags, warp, lane, it0, it1,
+                                                  rounds);
+  else if (FMT == kFmtInt8 && *reinterpret_cast<volatile const int*>(p.large_scale) != 0)
+    attn_consume<D, NG, NCW, R, NSTAGE, FMT, false, QT, SEL>(p, smem, stages, bar_base, cta_abort, tags, warp, lane,
+                                                         it0, it1, rounds);
   else
     attn_consume<D, NG, NCW, R, NSTAGE, FMT, true, QT, SEL>(p, smem, stages, bar_base, cta_abort, tags, warp,
                                                         lane, it0, it1, rounds);
@@ -1456,8 +1644,7 @@ cudaError_t launch_tc_r(const AttnParams& p, int grid, cudaStream_t stream) {
     default: break;
   }
   if (e != cudaSuccess || p.n_split_units == 0 || p.split_ctr != nullptr) return e;
-  attn_combine_kernel<D><<<p.n_split_units * p.Hkv, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return run_combine<D>(p, stream);
 }
 
 template <int D, int NG, int NCW, int R, int FMT>

@@ -22,19 +22,21 @@
 //                          kernel's shared-memory reads are conflict free
 //     [2*T*D, 4*T*D)       V transposed: D rows of T bf16
 //
-// 4-bit pools use sub-blocks of T = 64 tokens of T * (D + 8*NG) bytes:
-//     [0, 32*D)            K codes in the order of the decode kernel's MMA
+// 4-bit pools use sub-blocks of T = 64 tokens of T * (D + 8*NG) bytes, a K
+// half and a V half of 32*D + 256*NG bytes each (one bulk copy each):
+//     K half, [0, 32*D)    K codes in the order of the decode kernel's MMA
 //                          operand: 16-token x 16-element tiles of 32 lane
 //                          words, the four tiles of 64 elements interleaved so
 //                          that one 16-byte load per lane fetches them. Byte
 //                          (2h + hi) of word k holds the codes d (low nibble)
 //                          and d + 2 (high) of one token, d = 16c + 4k + h
-//     [32*D, 64*D)         V codes, tiles of 16 elements x 16 tokens, the four
+//             [32*D, ...)  K scales, K zeros: [NG][T] f16, token t at
+//                          (t % 8) * 8 + t / 8, so that the eight tokens of one
+//                          operand row are 16 consecutive bytes
+//     V half, [0, 32*D)    V codes, tiles of 16 elements x 16 tokens, the four
 //                          token tiles interleaved; a byte holds the codes d
 //                          and d + 8 of one token
-//     [64*D, ...)          K scales, K zeros, V scales, V zeros: [NG][T] f16,
-//                          token t at (t % 8) * 8 + t / 8, so that the eight
-//                          tokens of one operand row are 16 consecutive bytes
+//             [32*D, ...)  V scales, V zeros, as for K
 // Every code byte belongs to one token, so tokens are written independently.
 //
 // A pool with block summaries ends each page with spb rows of 2*D bytes (per
@@ -133,12 +135,14 @@ __host__ __device__ inline int q4_kbyte(int D, int t, int c, int j) {
   return ((((t >> 4) * (D >> 6) + (c >> 2)) * 32 + (t & 7) * 4 + (c & 3)) << 4) + (j >> 1) * 4 + (j & 1) * 2 +
          ((t >> 3) & 1);
 }
-__host__ __device__ inline int q4_vbyte(int D, int t, int c, int j) {
-  return 32 * D + ((c * 32 + j * 4 + ((t & 7) >> 1)) << 4) + (t >> 4) * 4 + (t & 1) * 2 + ((t >> 3) & 1);
+// Bytes of the K half, and of the V half that follows it.
+__host__ __device__ constexpr int q4_half(int D, int NG) { return 32 * D + 256 * NG; }
+__host__ __device__ inline int q4_vbyte(int D, int NG, int t, int c, int j) {
+  return q4_half(D, NG) + ((c * 32 + j * 4 + ((t & 7) >> 1)) << 4) + (t >> 4) * 4 + (t & 1) * 2 + ((t >> 3) & 1);
 }
 // meta array a (0 = K scale, 1 = K zero, 2 = V scale, 3 = V zero), group gi, token t
 __host__ __device__ inline int q4_meta(int D, int NG, int a, int gi, int t) {
-  return kSub4 * D + ((a * NG + gi) * kSub4 + (t & 7) * 8 + (t >> 3)) * 2;
+  return (a >> 1) * q4_half(D, NG) + 32 * D + (((a & 1) * NG + gi) * kSub4 + (t & 7) * 8 + (t >> 3)) * 2;
 }
 // Element of a 4-bit chunk held in the low nibble of its byte j, and the
 // distance to the one in the high nibble.

@@ -128,8 +128,9 @@ struct SubGeom {
   static constexpr int SB = FMT == kFmtBf16   ? T * 4 * D
                             : FMT == kFmtInt4 ? T * (D + 8 * NG)
                                               : T * (2 * D + 8 * NG);
-  static constexpr int VOFF = FMT == kFmtBf16 ? T * D * 2 : FMT == kFmtInt4 ? T * D / 2 : T * D;
-  static constexpr int META = FMT == kFmtInt4 ? T * D : 2 * T * D;  // int8 and int4
+  static constexpr int VOFF = FMT == kFmtBf16 ? T * D * 2 : FMT == kFmtInt4 ? q4_half(D, NG) : T * D;
+  static constexpr int META = 2 * T * D;     // int8 only
+  static constexpr int META4 = T * D / 2;    // int4: scales, then zeros, of a half
   // meta array a, group gi, token t -> byte offset (int8 only)
   static __device__ __forceinline__ int meta(int a, int gi, int t) {
     return META + ((a * NG + gi) * T + t) * 2;

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) append4_kernel(uint8_t* __restrict__ pool
   uint8_t* sb = pool + (((int64_t)d.block * geom.L + (layer_begin + li)) * geom.Hkv + h) * geom.page_bytes +
                 (int64_t)(slot / kSub4) * geom.sb_bytes;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, t, c, j)] = chunk_byte(codes, is_k, j);
+  for (int j = 0; j < 8; ++j) sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, NG, t, c, j)] = chunk_byte(codes, is_k, j);
   if (c % LPG == 0) {
     const int gi = c / LPG, a = is_k ? 0 : 2;
     *reinterpret_cast<uint16_t*>(sb + q4_meta(D, NG, a, gi, t)) = s16;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) append4_tile_kernel(uint8_t* __restrict__
     if (!live) continue;
     auto put = [&](uint8_t* to) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) to[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, t, c, j)] = chunk_byte(codes, is_k, j);
+      for (int j = 0; j < 8; ++j) to[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, NG, t, c, j)] = chunk_byte(codes, is_k, j);
       if (c % LPG == 0) {
         const int gi = c / LPG, a = is_k ? 0 : 2;
         *reinterpret_cast<uint16_t*>(to + q4_meta(D, NG, a, gi, t)) = s16;
@@ -258,10 +258,11 @@ __global__ void __launch_bounds__(256) append4_tile_kernel(uint8_t* __restrict__
 }
 
 // The 16 codes of chunk c of token t of a 4-bit sub-block.
-__device__ __forceinline__ void unpack_chunk(const uint8_t* sb, int D, int t, int c, bool is_k, uint8_t (&codes)[16]) {
+__device__ __forceinline__ void unpack_chunk(const uint8_t* sb, int D, int NG, int t, int c, bool is_k,
+                                             uint8_t (&codes)[16]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const uint8_t x = sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, t, c, j)];
+    const uint8_t x = sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, NG, t, c, j)];
     if (is_k) {
       codes[q4_elem(true, j)] = x & 15;
       codes[q4_elem(true, j) + q4_step(true)] = x >> 4;
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t* __restric
     float x[16];
     if (FMT == kFmtInt4) {
       uint8_t codes[16];
-      unpack_chunk(img, D, t, c, is_k, codes);
+      unpack_chunk(img, D, NG, t, c, is_k, codes);
       const float s = __half2float(*reinterpret_cast<const __half*>(img + q4_meta(D, NG, a, gi, t)));
       const float z = __half2float(*reinterpret_cast<const __half*>(img + q4_meta(D, NG, a + 1, gi, t)));
 #pragma unroll
@@ -370,7 +371,7 @@ __global__ void gather4_kernel(const uint8_t* __restrict__ pool, Geom geom, int 
   const uint16_t z16 = *reinterpret_cast<const uint16_t*>(sb + q4_meta(D, NG, a + 1, gi, t));
   if (dst) {
     uint8_t codes[16];
-    unpack_chunk(sb, D, t, c, is_k, codes);
+    unpack_chunk(sb, D, NG, t, c, is_k, codes);
     if (out.mode == 0) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) dst[orow * D + 16 * c + e] = codes[e];
@@ -410,7 +411,7 @@ __global__ void scatter4_kernel(uint8_t* __restrict__ pool, Geom geom, int layer
 #pragma unroll
   for (int e = 0; e < 16; ++e) codes[e] = src[e] & 15u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, t, c, j)] = chunk_byte(codes, is_k, j);
+  for (int j = 0; j < 8; ++j) sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, NG, t, c, j)] = chunk_byte(codes, is_k, j);
   if ((16 * c) % geom.G == 0) {
     const uint16_t s16 = (is_k ? in.key_scales : in.value_scales)[irow * NG + gi];
     *reinterpret_cast<uint16_t*>(sb + q4_meta(D, NG, a, gi, t)) = s16;

@@ -283,14 +283,15 @@ __device__ __forceinline__ void um_dequant4(const uint8_t* __restrict__ raw, uin
                                             uint8_t* __restrict__ vt, int t0, int valid) {
   using SG = SubGeom<D, NG, kFmtInt4>;
   constexpr int NDT = kUmDeqWarps * 32, NHH = D / 64, NK = 4 * NHH * 32, NV = D / 16 * 32;
-  const uint8_t* meta = raw + SG::META;
+  const uint8_t* kmeta = raw + SG::META4;              // + (scale 0, zero 1 * NG + group) * 128
+  const uint8_t* vmeta = raw + SG::VOFF + SG::META4;
   for (int i = t0; i < NK + NV; i += NDT) {
     const int lane = i & 31, r = lane >> 2, tig = lane & 3;
     if (i < NK) {
       const int hh = (i >> 5) % NHH, u = (i >> 5) / NHH, grp = 64 * hh / SG::G, t = 16 * u + r;
       const uint4 w4 = *reinterpret_cast<const uint4*>(raw + i * 16);
-      uint32_t s = *reinterpret_cast<const uint32_t*>(meta + grp * 128 + r * 16 + 4 * u);  // tokens t, t + 8
-      uint32_t z = *reinterpret_cast<const uint32_t*>(meta + (NG + grp) * 128 + r * 16 + 4 * u);
+      uint32_t s = *reinterpret_cast<const uint32_t*>(kmeta + grp * 128 + r * 16 + 4 * u);  // tokens t, t + 8
+      uint32_t z = *reinterpret_cast<const uint32_t*>(kmeta + (NG + grp) * 128 + r * 16 + 4 * u);
       if (valid < 64) {
         const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 8 < valid ? 0xffff0000u : 0u);
         s &= mk;
@@ -314,10 +315,10 @@ __device__ __forceinline__ void um_dequant4(const uint8_t* __restrict__ raw, uin
       const int v = i - NK, mt = v >> 5, grp = 16 * mt / SG::G, d = 16 * mt + r;
       const uint4 w4 = *reinterpret_cast<const uint4*>(raw + SG::VOFF + v * 16);
       // scales / zeros of the tokens 16u + 8hi + 2 tig (a) and + 1 (b)
-      const uint4 sa4 = *reinterpret_cast<const uint4*>(meta + (2 * NG + grp) * 128 + 32 * tig);
-      const uint4 sb4 = *reinterpret_cast<const uint4*>(meta + (2 * NG + grp) * 128 + 32 * tig + 16);
-      const uint4 za4 = *reinterpret_cast<const uint4*>(meta + (3 * NG + grp) * 128 + 32 * tig);
-      const uint4 zb4 = *reinterpret_cast<const uint4*>(meta + (3 * NG + grp) * 128 + 32 * tig + 16);
+      const uint4 sa4 = *reinterpret_cast<const uint4*>(vmeta + grp * 128 + 32 * tig);
+      const uint4 sb4 = *reinterpret_cast<const uint4*>(vmeta + grp * 128 + 32 * tig + 16);
+      const uint4 za4 = *reinterpret_cast<const uint4*>(vmeta + (NG + grp) * 128 + 32 * tig);
+      const uint4 zb4 = *reinterpret_cast<const uint4*>(vmeta + (NG + grp) * 128 + 32 * tig + 16);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
       const uint32_t sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w}, sb[4] = {sb4.x, sb4.y, sb4.z, sb4.w};
       const uint32_t za[4] = {za4.x, za4.y, za4.z, za4.w}, zb[4] = {zb4.x, zb4.y, zb4.z, zb4.w};
