@@ -131,7 +131,7 @@ struct Plan {
   std::vector<int32_t> gorder, gstart, gmembers, seq_sh;
   std::vector<int64_t> gshared;
   std::vector<ShItem> sh_items;
-  std::vector<int32_t> sh_members, sh_cta;
+  std::vector<int32_t> sh_members, sh_cta, sh_split;
   int last_C = 0, last_HG = 0, last_grid = 0;
   int64_t last_items = 0;
   int last_groups = 0, last_pslots = 0, last_sh_grid = 0;
@@ -892,6 +892,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   pl.sh_items.clear();
   pl.sh_members.clear();
   pl.sh_cta.clear();
+  pl.sh_split.clear();
   pl.pairs.clear();
   int n_pslots = 0, sh_grid = 0;
   {
@@ -932,6 +933,10 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   if (!pl.pairs.empty() && g.fmt == kFmtInt8 && p->cfg.attn_impl == KRILL_ATTN_TENSOR_CORE_PAIR && p->pair_slots > 0 &&
       shared_uses_umma(g, p->cfg.attn_impl))
     for (const Plan::Pair& pr : pl.pairs) sh_pair = sh_pair || pr.n_rows > 128;
+  // Causal items of the one-CTA kernel write their rows' outputs themselves;
+  // only row blocks cut at a CTA's end leave records (rows of row_rec_floats).
+  const bool direct = causal_path && !sh_pair;
+  int64_t rec_rows = 0;
   if (!pl.pairs.empty()) {
     int64_t W = 0;
     for (const Plan::Pair& pr : pl.pairs) W += pr.n_sb;
@@ -958,6 +963,11 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
         it.slot = (int16_t)(c - first);
         it.n_frag = (int16_t)(last - first + 1);
         it.causal = pr.causal;
+        if (direct && last > first) {
+          if (c == first) pl.sh_split.push_back((int32_t)pl.sh_items.size());
+          it.rec = (int32_t)rec_rows;
+          rec_rows += pr.n_rows;
+        }
         pl.sh_items.push_back(it);
         pl.sh_cta[(size_t)c + 1] += 1;
       }
@@ -978,6 +988,11 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   bool merge_in_kernel = latency_bound && !causal_path;
   for (int64_t ui = 0; ui < n_units; ++ui) {
     AttnUnit& u = pl.units[ui];
+    if (direct) {
+      u.first_split = 0;
+      u.n_split = 1;
+      continue;
+    }
     if (causal_path) {  // every record comes from the causal cascade items
       u.first_split = (int32_t)split_count;
       u.n_pre = 0;
@@ -1051,6 +1066,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   SelectParams selp{};
   if (sel) selp = select_params(p, *sel, q, q_dtype);
   if (!p->host_only) {
+    if (direct) split_count = (rec_rows * row_rec_floats(g.D) + partial_floats(g.D) - 1) / partial_floats(g.D) / g.Hkv + 1;
     TRY(ensure_scratch(p, split_count * g.Hkv, 0));
     if (sel) TRY(ensure_select(p, *sel, n_units * g.Hkv, max_n, &selp));
   }
@@ -1113,7 +1129,8 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   const size_t shm_bytes = align16(pl.sh_members.size() * sizeof(int32_t));
   const size_t sh_off = units_bytes + items_bytes + off_bytes + bt_bytes + su_bytes;
   // a deferred append's destinations ride in the same packet (one upload)
-  const size_t pre_off = sh_off + shi_bytes + shc_bytes + shm_bytes;
+  const size_t shs_bytes = align16(pl.sh_split.size() * sizeof(int32_t));
+  const size_t pre_off = sh_off + shi_bytes + shc_bytes + shm_bytes + shs_bytes;
   const size_t pre_bytes = pre && pre->pending ? align16(pre->dst.size() * sizeof(AppendDst)) : 0;
   const size_t total = pre_off + pre_bytes;
   StageSlot* slot = nullptr;
@@ -1147,6 +1164,9 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     std::memcpy(h + sh_off + shi_bytes, pl.sh_cta.data(), pl.sh_cta.size() * sizeof(int32_t));
     std::memcpy(h + sh_off + shi_bytes + shc_bytes, pl.sh_members.data(),
                 pl.sh_members.size() * sizeof(int32_t));
+    if (shs_bytes)
+      std::memcpy(h + sh_off + shi_bytes + shc_bytes + shm_bytes, pl.sh_split.data(),
+                  pl.sh_split.size() * sizeof(int32_t));
   }
   if (pre_bytes) std::memcpy(h + pre_off, pre->dst.data(), pre->dst.size() * sizeof(AppendDst));
   pl.last_groups = n_groups;
@@ -1169,6 +1189,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     dp.split_ctr = merge_in_kernel ? &ctr_tag : nullptr;
     dp.sh_grid = sh_grid;
     dp.sh_pair = sh_pair ? 1 : 0;
+    dp.n_sh_split = (int)pl.sh_split.size();
     static const int32_t sel_tag = 0;
     dp.sel = sel ? &sel_tag : nullptr;
     describe_attention(g, dp, grid, p->cfg.attn_impl, pl.last_kernels, sizeof(pl.last_kernels));
@@ -1215,6 +1236,9 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     ap.sh_grid = sh_grid;
     ap.sh_pair = sh_pair ? 1 : 0;
     ap.n_pslots = n_pslots;
+    ap.sh_direct = direct ? 1 : 0;
+    ap.sh_split = reinterpret_cast<const int32_t*>(slot->d + sh_off + shi_bytes + shc_bytes + shm_bytes);
+    ap.n_sh_split = (int)pl.sh_split.size();
   }
   if (pre_bytes) {
     const krill_status_t st =
@@ -1239,7 +1263,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   }
   CUDA_TRY(timed_launch(p, 0, stream, [&] { return launch_attention(g, ap, grid, p->cfg.attn_impl, stream); }));
   p->kernels += (grid > 0 ? 1 : 0) + (attn_needs_combine(ap, grid, p->cfg.attn_impl) ? 1 : 0) +
-                (sh_grid > 0 ? 1 : 0);
+                (sh_grid > 0 ? 1 : 0) + (pl.sh_split.empty() ? 0 : 1);
   TRY(stage_release(slot, stream));
   if (uses_scratch) {
     p->scratch_stream = stream;

@@ -93,11 +93,16 @@ struct ShItem {
   int16_t h;         // kv head
   int16_t slot;      // partial-record slot of this fragment
   int16_t n_frag;    // fragments of this (members, layer, head)
+  int32_t rec;       // direct causal items (see sh_direct): first row record of this
+                     // fragment; unused by the only fragment of its rows
   int32_t causal;    // -1: every row sees every token. Else the rows are the
                      // queries (row / g) of one sequence at positions causal +
                      // row / g, each seeing tokens up to its own (multi-query
                      // verify / chunked prefill)
 };
+
+// Row record of a direct causal fragment: O [D], the row's max and normalizer.
+__host__ __device__ constexpr int row_rec_floats(int D) { return D + 4; }
 
 // Query rows of one cascade item: 8 consumer warps x 32 rows (16 at D = 256,
 // whose fp32 output rows need twice the registers).
@@ -141,6 +146,13 @@ struct AttnParams {
   int sh_grid;                // CTAs, or CTA pairs when sh_pair (sh_cta_off per pair)
   int sh_pair;                // 1: the tcgen05 cascade runs as CTA pairs (cta_group::2)
   int n_pslots;               // prefix record slots per cascaded unit
+  // Direct causal items (single-CTA tcgen05 kernel): rows whose tokens are all
+  // in one fragment go straight to the output; the others' fragments write row
+  // records, which launch_row_combine merges (sh_split: each split row block's
+  // first item, its fragments' records n_rows apart).
+  int sh_direct;
+  const int32_t* sh_split;
+  int n_sh_split;
   // Block-sparse decode: the picked sub-blocks of (unit, kv head), ascending,
   // [units][Hkv][sel_stride]; unit items then index this list. nullptr: dense.
   const int32_t* sel;
@@ -244,6 +256,8 @@ bool shared_uses_umma(const Geom& g, int impl);
 // device at once (0: no pair kernel for this geometry, or no device).
 int shared_pair_capacity(const Geom& g);
 cudaError_t launch_shared_umma(const Geom& g, const AttnParams& p, cudaStream_t stream);
+// Merges the row records of split direct causal items (kv_shared_umma.cu).
+cudaError_t launch_row_combine(const Geom& g, const AttnParams& p, cudaStream_t stream);
 inline int shared_rows(const Geom& g, int impl) { return shared_uses_umma(g, impl) ? 256 : sh_rows(g.D); }
 // Launch description produced for the allocation-free decode attention:
 // byte offsets of the metadata and partial records inside the caller's

@@ -210,6 +210,8 @@ void describe_attention(const Geom& g, const AttnParams& p, int grid, int impl, 
     if (p.split_ctr != nullptr && p.n_split_units > 0 && impl != 1)
       put(snprintf(buf + n, cap - n, "[merge in kernel]"));
   }
+  if (p.n_sh_split > 0)
+    put(snprintf(buf + n, cap - n, "%srow_combine_kernel<%d>", n > 0 && buf[n - 1] != '+' ? "+" : "", g.D));
   if (attn_needs_combine(p, grid, impl))
     put(snprintf(buf + n, cap - n, "%sattn_combine_kernel<%d>", n > 0 && buf[n - 1] != '+' ? "+" : "", g.D));
   if (n > 0 && buf[n - 1] == '+') buf[--n] = 0;
@@ -222,6 +224,7 @@ cudaError_t launch_attention(const Geom& g, const AttnParams& p, int grid, int i
                                                     : launch_shared(g, p, stream);
     if (e != cudaSuccess) return e;
   }
+  if (p.sh_direct) return launch_row_combine(g, p, stream);
   if (grid <= 0) return launch_combine(g, p, stream);  // everything was in cascade items
   if (impl == 1) {  // KRILL_ATTN_CUDA_CORE
     if (g.D == 64 && g.NG == 1) return launch_cc<64, 1>(p, grid, stream);

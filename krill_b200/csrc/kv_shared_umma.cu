@@ -353,6 +353,67 @@ __device__ __forceinline__ float max64(const float (&a)[32], const float (&b)[32
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
+// 32 consecutive outputs o * inv of one row (64-byte aligned at least).
+__device__ __forceinline__ void store_out32(void* out, int dtype, int64_t at, const float (&o)[32], float inv) {
+  if (dtype == KRILL_DTYPE_F32) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      dst[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+    return;
+  }
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = o[8 * i + 2 * k] * inv, b = o[8 * i + 2 * k + 1] * inv;
+      if (dtype == KRILL_DTYPE_F16) {
+        w[k] = f2h2(a, b);
+      } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        w[k] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Merges the fragments of split row blocks of direct causal items: one warp
+// per query row, lanes over D, records in fragment order.
+template <int D>
+__global__ void __launch_bounds__(256) row_combine_kernel(AttnParams p) {
+  constexpr int V = D / 32;
+  const int lane = threadIdx.x & 31;
+  const ShItem item = p.sh_items[p.sh_split[blockIdx.y]];
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= item.n_rows) return;
+  const float* rec = p.partials + (int64_t)(item.rec + row) * row_rec_floats(D);
+  const int64_t stride = (int64_t)item.n_rows * row_rec_floats(D);
+  float M = -INFINITY;
+  for (int i = 0; i < item.n_frag; ++i) M = fmaxf(M, rec[i * stride + D]);
+  float Ls = 0.f, Os[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) Os[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < item.n_frag; ++i) {
+    const float mi = rec[i * stride + D], li = rec[i * stride + D + 1];
+    const float w = mi == -INFINITY ? 0.f : exp2f(mi - M);
+    Ls += (mi == -INFINITY) ? 0.f : li * w;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float oi = rec[i * stride + lane + 32 * e];
+      Os[e] = (mi != -INFINITY) ? Os[e] + oi * w : Os[e];
+    }
+  }
+  const float inv = 1.f / Ls;
+  const AttnUnit* un = p.units + p.sh_members[item.mem_off + row / p.g];
+  const int64_t orow = ((int64_t)un->qo_row * p.Hq + (int64_t)item.h * p.g + row % p.g) * D;
+#pragma unroll
+  for (int e = 0; e < V; ++e) store_out(p.out, p.out_dtype, orow + lane + 32 * e, Os[e] * inv);
+}
+
 template <int D, int NG, int FMT>
 __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnParams p) {
   using SM = UmSmem<D, NG, FMT>;
@@ -693,25 +754,39 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
         float* part = nullptr;
         int jq = 0;
         const AttnUnit* un = nullptr;
+        const bool whole = p.sh_direct && item.n_frag == 1;  // the row's result is complete
+        int64_t orow = 0;
         if (row < item.n_rows) {
           const int mem = row / gq;
           jq = row - mem * gq;
           un = p.units + p.sh_members[item.mem_off + mem];
-          part = p.partials +
-                 ((int64_t)(un->first_split + item.slot) * Hkv + item.h) * partial_floats(D);
+          if (whole)
+            orow = ((int64_t)un->qo_row * p.Hq + (int64_t)item.h * gq + jq) * D;
+          else if (p.sh_direct)
+            part = p.partials + (int64_t)(item.rec + row) * row_rec_floats(D);
+          else
+            part = p.partials +
+                   ((int64_t)(un->first_split + item.slot) * Hkv + item.h) * partial_floats(D) + 16 + jq * D;
         }
+        const float inv = whole ? 1.f / l : 0.f;
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
           float o[32];
           tmem_ld32(lane_addr + 32u * cc, o);
           if (part) {
-            float4* dst = reinterpret_cast<float4*>(part + 16 + jq * D + 32 * cc);
+            float4* dst = reinterpret_cast<float4*>(part + 32 * cc);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else if (whole && row < item.n_rows) {
+            store_out32(p.out, p.out_dtype, orow + 32 * cc, o, inv);
           }
         }
-        if (part) {
+        if (part && p.sh_direct) {
+          part[D] = m;
+          part[D + 1] = l;
+        } else if (part) {
+          part -= 16 + jq * D;
           part[jq] = m;
           part[8 + jq] = l;
           if (item.slot == 0)
@@ -1411,6 +1486,14 @@ int shared_pair_capacity(const Geom& g) {
   if (g.D == 128 && g.NG == 2) return pair_capacity<128, 2>();
   if (g.D == 128 && g.NG == 1) return pair_capacity<128, 1>();
   return 0;
+}
+
+cudaError_t launch_row_combine(const Geom& g, const AttnParams& p, cudaStream_t stream) {
+  if (p.n_sh_split == 0) return cudaSuccess;
+  const dim3 grid(256 / 8, (unsigned)p.n_sh_split);
+  if (g.D == 64) row_combine_kernel<64><<<grid, 256, 0, stream>>>(p);
+  else row_combine_kernel<128><<<grid, 256, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_shared_umma(const Geom& g, const AttnParams& p, cudaStream_t stream) {
