@@ -560,7 +560,7 @@ __device__ __forceinline__ uint32_t q4_word(const uint4& w, int u) {
 __device__ __forceinline__ float2 q4_pair(const uint4& w, int u) { return __half22float2(u2h(q4_word(w, u))); }
 
 // tc_subblock for 4-bit pools in two parts (same arguments; row r of token
-// tile u is token 16u + r, rows r + 8 the tokens 8 further): the K half gives
+// tile u is token 16 (r / 2) + 4u + r % 2, rows r + 8 the tokens 2 further): the K half gives
 // the scores s and, after the online softmax, p * 2^bias in their place, the
 // f16 pairs ph and the rescale al of what came before; the V half adds P.V.
 // ILV token tiles (K) or row tiles (V) advance together, so that consecutive
@@ -633,7 +633,7 @@ __device__ __forceinline__ void q4_scores(const uint8_t* __restrict__ sb, TCStat
     for (int q = 0; q < QT; ++q)
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int pa = pos0 + 16 * u + r, pb = pa + 8;
+        const int pa = pos0 + 16 * (r >> 1) + 4 * u + (r & 1), pb = pa + 2;
         if (pa < t_lo || pa >= th[q][0]) s[q][u][0] = -INFINITY;
         if (pa < t_lo || pa >= th[q][1]) s[q][u][1] = -INFINITY;
         if (pb < t_lo || pb >= th[q][0]) s[q][u][2] = -INFINITY;
@@ -704,7 +704,7 @@ __device__ __forceinline__ void q4_weights(const uint8_t* __restrict__ vb, Q4Sta
       uint32_t mk[4];
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int pa = pos0 + 16 * u + r, pc = pa + 8;
+        const int pa = pos0 + 16 * (r >> 1) + 4 * u + (r & 1), pc = pa + 2;
         mk[u] = ((pa >= t_lo && pa < t_hi) ? 0x0000ffffu : 0u) | ((pc >= t_lo && pc < t_hi) ? 0xffff0000u : 0u);
       }
       vsw = make_uint4(vsw.x & mk[0], vsw.y & mk[1], vsw.z & mk[2], vsw.w & mk[3]);

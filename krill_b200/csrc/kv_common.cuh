@@ -24,15 +24,18 @@
 //
 // 4-bit pools use sub-blocks of T = 64 tokens of T * (D + 8*NG) bytes, a K
 // half and a V half of 32*D + 256*NG bytes each (one bulk copy each):
+// Token t of a sub-block is row r (hi = 0) or r + 8 (hi = 1) of the 16-token
+// tile u, with t = 16 (r / 2) + 4 u + 2 hi + r % 2: a lane of the V operand then
+// holds 16 consecutive tokens over the four tiles.
 //     K half, [0, 32*D)    K codes in the order of the decode kernel's MMA
 //                          operand: 16-token x 16-element tiles of 32 lane
 //                          words, the four tiles of 64 elements interleaved so
 //                          that one 16-byte load per lane fetches them. Byte
 //                          (2h + hi) of word k holds the codes d (low nibble)
 //                          and d + 2 (high) of one token, d = 16c + 4k + h
-//             [32*D, ...)  K scales, K zeros: [NG][T] f16, token t at
-//                          (t % 8) * 8 + t / 8, so that the eight tokens of one
-//                          operand row are 16 consecutive bytes
+//             [32*D, ...)  K scales, K zeros: [NG][T] f16, token at 8 r + 2 u +
+//                          hi, so that the eight tokens of one operand row are
+//                          16 consecutive bytes
 //     V half, [0, 32*D)    V codes, tiles of 16 elements x 16 tokens, the four
 //                          token tiles interleaved; a byte holds the codes d
 //                          and d + 8 of one token
@@ -129,20 +132,24 @@ __host__ __device__ inline int64_t raw_voff(int D, int T, int t, int d) {
   return ((int64_t)T * D + (int64_t)d * T + t) * 2;
 }
 
+// Tile, row and half of a token of a 4-bit sub-block (see above).
+__host__ __device__ constexpr int q4_tile(int t) { return (t >> 2) & 3; }
+__host__ __device__ constexpr int q4_row(int t) { return ((t >> 4) << 1) | (t & 1); }
+__host__ __device__ constexpr int q4_hi(int t) { return (t >> 1) & 1; }
 // 4-bit sub-block: byte j (0..7) of 16-element chunk c of token t. K: codes
 // d = 16c + 4(j/2) + j%2 (low nibble) and d + 2; V: codes d = 16c + j and d + 8.
 __host__ __device__ inline int q4_kbyte(int D, int t, int c, int j) {
-  return ((((t >> 4) * (D >> 6) + (c >> 2)) * 32 + (t & 7) * 4 + (c & 3)) << 4) + (j >> 1) * 4 + (j & 1) * 2 +
-         ((t >> 3) & 1);
+  return (((q4_tile(t) * (D >> 6) + (c >> 2)) * 32 + q4_row(t) * 4 + (c & 3)) << 4) + (j >> 1) * 4 + (j & 1) * 2 +
+         q4_hi(t);
 }
 // Bytes of the K half, and of the V half that follows it.
 __host__ __device__ constexpr int q4_half(int D, int NG) { return 32 * D + 256 * NG; }
 __host__ __device__ inline int q4_vbyte(int D, int NG, int t, int c, int j) {
-  return q4_half(D, NG) + ((c * 32 + j * 4 + ((t & 7) >> 1)) << 4) + (t >> 4) * 4 + (t & 1) * 2 + ((t >> 3) & 1);
+  return q4_half(D, NG) + ((c * 32 + j * 4 + (t >> 4)) << 4) + q4_tile(t) * 4 + (t & 1) * 2 + q4_hi(t);
 }
 // meta array a (0 = K scale, 1 = K zero, 2 = V scale, 3 = V zero), group gi, token t
 __host__ __device__ inline int q4_meta(int D, int NG, int a, int gi, int t) {
-  return (a >> 1) * q4_half(D, NG) + 32 * D + (((a & 1) * NG + gi) * kSub4 + (t & 7) * 8 + (t >> 3)) * 2;
+  return (a >> 1) * q4_half(D, NG) + 32 * D + (((a & 1) * NG + gi) * kSub4 + q4_row(t) * 8 + q4_tile(t) * 2 + q4_hi(t)) * 2;
 }
 // Element of a 4-bit chunk held in the low nibble of its byte j, and the
 // distance to the one in the high nibble.

@@ -28,6 +28,19 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t phase) 
       : "memory");
   return done;
 }
+// Non-blocking form, for a warp that polls several barriers (try_wait may
+// suspend it on one while another completes).
+__device__ __forceinline__ uint32_t mbar_test_wait(uint32_t bar, uint32_t phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(phase)
+      : "memory");
+  return done;
+}
 __device__ __forceinline__ uint64_t globaltimer() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));

@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __r
   const uint8_t* sb = page + (int64_t)it.sub * geom.sb_bytes;
   int subsets;
   if (FMT == kFmtInt4) {
-    // warp w takes token tile w; lane (r, tig) the tokens r and r + 8 and the
+    // warp w takes token tile w; lane (r, tig) the tile's rows r and r + 8 and the
     // channels 16 tig .. + 15 of each run of 64
     subsets = 4;
     const int r = lane >> 2, tig = lane & 3, u = warp;
@@ -42,8 +42,8 @@ __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __r
       const int gi = 64 * hh / geom.G;
       const uint4 w4 = *reinterpret_cast<const uint4*>(sb + ((u * (D / 64) + hh) * 32 + lane) * 16);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      const float2 s = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(sb + q4_meta(D, NG, 0, gi, 16 * u + r))));
-      const float2 z = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(sb + q4_meta(D, NG, 1, gi, 16 * u + r))));
+      const float2 s = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(sb + q4_meta(D, NG, 0, gi, 0) + (8 * r + 2 * u) * 2)));
+      const float2 z = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(sb + q4_meta(D, NG, 1, gi, 0) + (8 * r + 2 * u) * 2)));
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int k = e >> 2, sh = (e & 1) * 16 + ((e >> 1) & 1) * 4;  // d = 4k + h + 2 * high nibble

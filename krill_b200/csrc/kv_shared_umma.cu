@@ -10,8 +10,8 @@
 //   - warps 10-19 dequantize each raw sub-block once (int8: the reference's two
 //     fp16 roundings; 4-bit pools: one fma) into f16 K [64 tok][D] and V [D][64 tok] tiles laid out
 //     as the tensor core's canonical K-major 128-byte-swizzled operands;
-//   - warp 8 owns the tensor memory (512 columns) and one of its lanes issues
-//     the MMAs, per half h:
+//   - warp 8 owns the tensor memory (512 columns) and an elected lane of it
+//     issues the MMAs, per half h:
 //       S_h  = Q_h · K_jᵀ     (M = 128 query rows, N = 64 tokens, K = D)
 //       O_h += P_h · V_j      (M = 128, N = D, K = 64 tokens)
 //     with S double-buffered in tensor memory so the softmax of tile j
@@ -162,10 +162,11 @@ struct UmSmem {
   static constexpr int KV_STAGE = K_BYTES + V_BYTES;
   static constexpr int RAW_OFF = KV_OFF + kUmNF * KV_STAGE;
   static constexpr int BAR_OFF = RAW_OFF + kUmNR * SG::SB;
-  // raw full/empty [NR], kv full/empty [NF]; per half: s full [2], p full,
-  // pv done, q full; fin
+  // raw full/empty [NR], k full/empty and v full/empty [NF]; per half: s full
+  // [2], p full, pv done, q full; fin
   static constexpr int B_RF = 0, B_RE = kUmNR, B_KF = 2 * kUmNR, B_KE = 2 * kUmNR + kUmNF,
-                       B_SF = 2 * kUmNR + 2 * kUmNF,  // [half][2]
+                       B_VF = 2 * kUmNR + 2 * kUmNF, B_VE = 2 * kUmNR + 3 * kUmNF,
+                       B_SF = 2 * kUmNR + 4 * kUmNF,  // [half][2]
                        B_PF = B_SF + 4, B_PD = B_PF + 2, B_QF = B_PD + 2, B_FIN = B_QF + 2,
                        NBAR = B_FIN + 1;
   static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;  // tmem address, abort flag
@@ -269,76 +270,87 @@ __device__ __forceinline__ void um_dequant(const uint8_t* __restrict__ raw, uint
   }
 }
 
-// um_dequant for 4-bit pools: values f16(code * scale + zero), one fma per
-// pair. A K item is a lane word group of the sub-block (tokens r and r + 8, 16
-// elements each, in order), a V item one of four token tiles (two rows d, d +
-// 8, pairs of tokens). Tokens at or past `valid` read as zero, whatever the
-// sub-block holds there.
+// um_dequant for 4-bit pools, K and V apart: values f16(code * scale + zero),
+// one fma per pair. An item is one lane word group of the sub-block. K: the
+// tokens of rows r and r + 8 of a tile, 16 consecutive elements each; V: rows d
+// and d + 8, 16 consecutive tokens. Tokens at or past `valid` read as zero,
+// whatever the sub-block holds there.
 __device__ __forceinline__ uint32_t deq4(uint32_t w, uint32_t s2, uint32_t z2) {
   const __half2 c = __hsub2_rn(u2h((w & 0x000f000fu) | 0x64006400u), u2h(0x64006400u));  // 1024 + c - 1024
   return h2u(__hfma2(c, u2h(s2), u2h(z2)));
 }
 template <int D, int NG>
-__device__ __forceinline__ void um_dequant4(const uint8_t* __restrict__ raw, uint8_t* __restrict__ kt,
-                                            uint8_t* __restrict__ vt, int t0, int valid) {
+__device__ __forceinline__ void um_dequant4_k(const uint8_t* __restrict__ raw, uint8_t* __restrict__ kt, int t0,
+                                              int valid) {
   using SG = SubGeom<D, NG, kFmtInt4>;
-  constexpr int NDT = kUmDeqWarps * 32, NHH = D / 64, NK = 4 * NHH * 32, NV = D / 16 * 32;
-  const uint8_t* kmeta = raw + SG::META4;              // + (scale 0, zero 1 * NG + group) * 128
-  const uint8_t* vmeta = raw + SG::VOFF + SG::META4;
-  for (int i = t0; i < NK + NV; i += NDT) {
+  constexpr int NHH = D / 64;
+  const uint8_t* meta = raw + SG::META4;
+  for (int i = t0; i < 4 * NHH * 32; i += kUmDeqWarps * 32) {
     const int lane = i & 31, r = lane >> 2, tig = lane & 3;
-    if (i < NK) {
-      const int hh = (i >> 5) % NHH, u = (i >> 5) / NHH, grp = 64 * hh / SG::G, t = 16 * u + r;
-      const uint4 w4 = *reinterpret_cast<const uint4*>(raw + i * 16);
-      uint32_t s = *reinterpret_cast<const uint32_t*>(kmeta + grp * 128 + r * 16 + 4 * u);  // tokens t, t + 8
-      uint32_t z = *reinterpret_cast<const uint32_t*>(kmeta + (NG + grp) * 128 + r * 16 + 4 * u);
-      if (valid < 64) {
-        const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 8 < valid ? 0xffff0000u : 0u);
-        s &= mk;
-        z &= mk;
+    const int hh = (i >> 5) % NHH, u = (i >> 5) / NHH, grp = 64 * hh / SG::G;
+    const int t = 16 * (r >> 1) + 4 * u + (r & 1);
+    const uint4 w4 = *reinterpret_cast<const uint4*>(raw + i * 16);
+    uint32_t s = *reinterpret_cast<const uint32_t*>(meta + grp * 128 + r * 16 + 4 * u);  // tokens t, t + 2
+    uint32_t z = *reinterpret_cast<const uint32_t*>(meta + (NG + grp) * 128 + r * 16 + 4 * u);
+    if (valid < 64) {
+      const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 2 < valid ? 0xffff0000u : 0u);
+      s &= mk;
+      z &= mk;
+    }
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) {
+      const uint32_t s2 = __byte_perm(s, 0, hi ? 0x3232 : 0x1010), z2 = __byte_perm(z, 0, hi ? 0x3232 : 0x1010);
+      uint32_t o[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[2 * k] = deq4(w[k] >> (8 * hi), s2, z2);
+        o[2 * k + 1] = deq4(w[k] >> (8 * hi + 4), s2, z2);
       }
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      const int c = 2 * (4 * hh + tig);
+      *reinterpret_cast<uint4*>(kt + sw128_off(64, t + 2 * hi, c)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(kt + sw128_off(64, t + 2 * hi, c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  }
+}
+template <int D, int NG>
+__device__ __forceinline__ void um_dequant4_v(const uint8_t* __restrict__ raw, uint8_t* __restrict__ vt, int t0,
+                                              int valid) {
+  using SG = SubGeom<D, NG, kFmtInt4>;
+  const uint8_t* meta = raw + SG::VOFF + SG::META4;
+  for (int i = t0; i < D / 16 * 32; i += kUmDeqWarps * 32) {
+    const int lane = i & 31, r = lane >> 2, tig = lane & 3, mt = i >> 5, grp = 16 * mt / SG::G, d = 16 * mt + r;
+    const uint4 w4 = *reinterpret_cast<const uint4*>(raw + SG::VOFF + i * 16);
+    // scales / zeros of the tokens 16 tig + 4u + 2hi (a) and + 1 (b)
+    const uint4 sa4 = *reinterpret_cast<const uint4*>(meta + grp * 128 + 32 * tig);
+    const uint4 sb4 = *reinterpret_cast<const uint4*>(meta + grp * 128 + 32 * tig + 16);
+    const uint4 za4 = *reinterpret_cast<const uint4*>(meta + (NG + grp) * 128 + 32 * tig);
+    const uint4 zb4 = *reinterpret_cast<const uint4*>(meta + (NG + grp) * 128 + 32 * tig + 16);
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    const uint32_t sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w}, sb[4] = {sb4.x, sb4.y, sb4.z, sb4.w};
+    const uint32_t za[4] = {za4.x, za4.y, za4.z, za4.w}, zb[4] = {zb4.x, zb4.y, zb4.z, zb4.w};
+    uint32_t o[2][8];  // rows d and d + 8
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int hi = 0; hi < 2; ++hi) {
-        const uint32_t s2 = __byte_perm(s, 0, hi ? 0x3232 : 0x1010), z2 = __byte_perm(z, 0, hi ? 0x3232 : 0x1010);
-        uint32_t o[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          o[2 * k] = deq4(w[k] >> (8 * hi), s2, z2);
-          o[2 * k + 1] = deq4(w[k] >> (8 * hi + 4), s2, z2);
+        uint32_t s2 = __byte_perm(sa[u], sb[u], hi ? 0x7632 : 0x5410);
+        uint32_t z2 = __byte_perm(za[u], zb[u], hi ? 0x7632 : 0x5410);
+        if (valid < 64) {
+          const int t = 16 * tig + 4 * u + 2 * hi;
+          const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 1 < valid ? 0xffff0000u : 0u);
+          s2 &= mk;
+          z2 &= mk;
         }
-        const int c = 2 * (4 * hh + tig);
-        *reinterpret_cast<uint4*>(kt + sw128_off(64, t + 8 * hi, c)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(kt + sw128_off(64, t + 8 * hi, c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+        o[0][2 * u + hi] = deq4(w[u] >> (8 * hi), s2, z2);
+        o[1][2 * u + hi] = deq4(w[u] >> (8 * hi + 4), s2, z2);
       }
-    } else {
-      const int v = i - NK, mt = v >> 5, grp = 16 * mt / SG::G, d = 16 * mt + r;
-      const uint4 w4 = *reinterpret_cast<const uint4*>(raw + SG::VOFF + v * 16);
-      // scales / zeros of the tokens 16u + 8hi + 2 tig (a) and + 1 (b)
-      const uint4 sa4 = *reinterpret_cast<const uint4*>(vmeta + grp * 128 + 32 * tig);
-      const uint4 sb4 = *reinterpret_cast<const uint4*>(vmeta + grp * 128 + 32 * tig + 16);
-      const uint4 za4 = *reinterpret_cast<const uint4*>(vmeta + (NG + grp) * 128 + 32 * tig);
-      const uint4 zb4 = *reinterpret_cast<const uint4*>(vmeta + (NG + grp) * 128 + 32 * tig + 16);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      const uint32_t sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w}, sb[4] = {sb4.x, sb4.y, sb4.z, sb4.w};
-      const uint32_t za[4] = {za4.x, za4.y, za4.z, za4.w}, zb[4] = {zb4.x, zb4.y, zb4.z, zb4.w};
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int hi = 0; hi < 2; ++hi) {
-          uint32_t s2 = __byte_perm(sa[u], sb[u], hi ? 0x7632 : 0x5410);
-          uint32_t z2 = __byte_perm(za[u], zb[u], hi ? 0x7632 : 0x5410);
-          if (valid < 64) {
-            const int t = 16 * u + 8 * hi + 2 * tig;
-            const uint32_t mk = (t < valid ? 0x0000ffffu : 0u) | (t + 1 < valid ? 0xffff0000u : 0u);
-            s2 &= mk;
-            z2 &= mk;
-          }
-          *reinterpret_cast<uint32_t*>(vt + sw128_off(D, d, 2 * u + hi) + 4 * tig) = deq4(w[u] >> (8 * hi), s2, z2);
-          *reinterpret_cast<uint32_t*>(vt + sw128_off(D, d + 8, 2 * u + hi) + 4 * tig) =
-              deq4(w[u] >> (8 * hi + 4), s2, z2);
-        }
-    }
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint4*>(vt + sw128_off(D, d + 8 * b, 2 * tig + c)) =
+            make_uint4(o[b][4 * c], o[b][4 * c + 1], o[b][4 * c + 2], o[b][4 * c + 3]);
   }
 }
 
@@ -441,6 +453,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
     for (int s = 0; s < kUmNF; ++s) {
       mbar_init(bar(SM::B_KF + s), kUmDeqWarps);
       mbar_init(bar(SM::B_KE + s), 1);            // MMA commit
+      mbar_init(bar(SM::B_VF + s), kUmDeqWarps);
+      mbar_init(bar(SM::B_VE + s), 1);            // MMA commit
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(bar(SM::B_SF + 2 * h), 1);        // MMA commit
@@ -502,25 +516,49 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
       for (int j = item.sb_begin; j < item.sb_end; ++j, ++J) {
         const uint32_t rs = J % kUmNR, fs = J % kUmNF;
         mbar_wait(bar(SM::B_RF + rs), (J / kUmNR) & 1, cta_abort, p.err);
-        if (J >= (uint32_t)kUmNF)
-          mbar_wait(bar(SM::B_KE + fs), ((J / kUmNF) - 1) & 1, cta_abort, p.err);
+        // K and V tiles have stages of their own: K of a tile is free once S of
+        // it is done, and S needs no more than K, so the K part (dequantized
+        // first) runs ahead of the softmax
         uint8_t* kt = smem + SM::KV_OFF + fs * SM::KV_STAGE;
-        if constexpr (FMT == kFmtInt4)  // tokens past the last query's position count as zero
-          um_dequant4<D, NG>(smem + SM::RAW_OFF + rs * SB, kt, kt + SM::K_BYTES, t0,
-                             item.causal < 0 ? 64 : item.causal + (item.n_rows - 1) / p.g + 1 - 64 * j);
-        else
-          um_dequant<D, NG>(smem + SM::RAW_OFF + rs * SB, kt, kt + SM::K_BYTES, t0);
+        const uint8_t* raw = smem + SM::RAW_OFF + rs * SB;
+        auto wait_free = [&](int b0) {
+          if (J >= (uint32_t)kUmNF) mbar_wait(bar(b0 + fs), ((J / kUmNF) - 1) & 1, cta_abort, p.err);
+        };
+        if constexpr (FMT == kFmtInt4) {  // tokens past the last query's position count as zero
+          const int valid = item.causal < 0 ? 64 : item.causal + (item.n_rows - 1) / p.g + 1 - 64 * j;
+          wait_free(SM::B_KE);
+          um_dequant4_k<D, NG>(raw, kt, t0, valid);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(SM::B_KF + fs));
+          wait_free(SM::B_VE);
+          um_dequant4_v<D, NG>(raw, kt + SM::K_BYTES, t0, valid);
+        } else {
+          wait_free(SM::B_KE);
+          wait_free(SM::B_VE);
+          um_dequant<D, NG>(raw, kt, kt + SM::K_BYTES, t0);
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(bar(SM::B_RE + rs));
-          mbar_arrive(bar(SM::B_KF + fs));
+          if (FMT != kFmtInt4) mbar_arrive(bar(SM::B_KF + fs));
+          mbar_arrive(bar(SM::B_VF + fs));
         }
       }
     }
   } else {
     // ---------------- MMA issuer (warp 8) ----------------
-    if (lane == 0) {
+    // The whole warp runs the loop and an elected lane issues: control flow and
+    // descriptors are then warp-uniform and stay in uniform registers (issued
+    // from a branch that one lane had taken, an MMA cost 140 cycles of the
+    // issuing warp, twice what the tensor core needs for it).
+    {
+      uint32_t leader;
+      asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+      auto ready = [&](uint32_t b, uint32_t phase) {
+        return __any_sync(0xffffffffu, mbar_test_wait(b, phase) != 0);
+      };
       constexpr uint32_t idS = umma_idesc(128, 64), idO = umma_idesc(128, D);
       uint32_t cnt0 = 0, cnt1 = 0;  // tiles processed by each half
       uint32_t qn0 = 0, qn1 = 0;    // items processed by each half
@@ -554,8 +592,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
           ++qn1;
         }
         tc_fence_after();
-        // S of tile js goes out once its K/V tiles are ready and its S buffer
-        // has been read (the softmax of tile js-2 is done, i.e. P·V of js-2 was
+        // S of tile js goes out once its K tile is ready and its S buffer has
+        // been read (the softmax of tile js-2 is done, i.e. P·V of js-2 was
         // issued); P·V of tile jp once both halves' P are ready. Whichever is
         // ready first is issued, so neither chain waits on the other.
         int js = 0, jp = 0;
@@ -565,33 +603,41 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
           bool progressed = false;
           if (js < n && js <= jp + 1) {
             const uint32_t Jc = J + js, st = Jc % kUmNF;
-            if (mbar_try_wait(bar(SM::B_KF + st), (Jc / kUmNF) & 1)) {
+            if (ready(bar(SM::B_KF + st), (Jc / kUmNF) & 1)) {
               tc_fence_after();
               const uint64_t kd = dK0 + (uint64_t)(st * (SM::KV_STAGE >> 4));
+              if (leader) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if (h >= nh) break;
-                const uint32_t c = (h == 0 ? cnt0 : cnt1) + js;
-                const uint64_t qd = dQ0 + (uint64_t)(h * (SM::QH_BYTES >> 4));
-                const uint32_t sc = tmem + 256u * h + kUmS0 + 64u * (c & 1);
+                for (int h = 0; h < 2; ++h) {
+                  if (h >= nh) break;
+                  const uint32_t c = (h == 0 ? cnt0 : cnt1) + js;
+                  const uint64_t qd = dQ0 + (uint64_t)(h * (SM::QH_BYTES >> 4));
+                  const uint32_t sc = tmem + 256u * h + kUmS0 + 64u * (c & 1);
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                  umma_f16(sc, qd + (uint64_t)(((ks >> 2) * (128 * 128) + 32 * (ks & 3)) >> 4),
-                           kd + (uint64_t)(((ks >> 2) * (64 * 128) + 32 * (ks & 3)) >> 4), idS,
-                           ks > 0 ? 1u : 0u);
-                umma_commit(bar(SM::B_SF + 2 * h + (c & 1)));
+                  for (int ks = 0; ks < D / 16; ++ks)
+                    umma_f16(sc, qd + (uint64_t)(((ks >> 2) * (128 * 128) + 32 * (ks & 3)) >> 4),
+                             kd + (uint64_t)(((ks >> 2) * (64 * 128) + 32 * (ks & 3)) >> 4), idS,
+                             ks > 0 ? 1u : 0u);
+                  umma_commit(bar(SM::B_SF + 2 * h + (c & 1)));
+                }
+                umma_commit(bar(SM::B_KE + st));  // K stage free
               }
+              __syncwarp();
               ++js;
               progressed = true;
             }
           }
-          if (jp < js && mbar_try_wait(bar(SM::B_PF), (cnt0 + jp) & 1) &&
-              (nh < 2 || mbar_try_wait(bar(SM::B_PF + 1), (cnt1 + jp) & 1))) {
+          if (jp < js && ready(bar(SM::B_PF), (cnt0 + jp) & 1) &&
+              (nh < 2 || ready(bar(SM::B_PF + 1), (cnt1 + jp) & 1)) &&
+              ready(bar(SM::B_VF + (J + jp) % kUmNF), ((J + jp) / kUmNF) & 1)) {
             tc_fence_after();
             const uint32_t st = (J + jp) % kUmNF;
-            issue_pv(0, st, jp == 0);
-            if (nh > 1) issue_pv(1, st, jp == 0);
-            umma_commit(bar(SM::B_KE + st));  // K/V stage free
+            if (leader) {
+              issue_pv(0, st, jp == 0);
+              if (nh > 1) issue_pv(1, st, jp == 0);
+              umma_commit(bar(SM::B_VE + st));  // V stage free
+            }
+            __syncwarp();
             ++jp;
             progressed = true;
           }
@@ -601,9 +647,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
           } else if ((++spins & 63u) == 0) {  // bounded: no progress within the pool's wait limit
             const uint64_t now = globaltimer();
             if (idle_since == 0) idle_since = now;
-            if (((now - idle_since) >> 10) > wait_limit_units(cta_abort)) {
+            if (__any_sync(0xffffffffu, ((now - idle_since) >> 10) > wait_limit_units(cta_abort))) {
               *cta_abort = 1;
-              atomicOr(p.err, kErrTimeout);
+              if (leader) atomicOr(p.err, kErrTimeout);
               break;
             }
           }
@@ -613,7 +659,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
         J += (uint32_t)n;
       }
       // every MMA has completed before the tensor memory is released
-      umma_commit(bar(SM::B_FIN));
+      if (leader) umma_commit(bar(SM::B_FIN));
       mbar_wait(bar(SM::B_FIN), 0, cta_abort, p.err);
     }
   }
@@ -660,6 +706,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(SM::B_QF + h));
       }
+      const int own_pos = item.causal + row / gq;  // causal items: this row's position
       float m = -INFINITY, l = 0.f;
       uint8_t* pb = smem + SM::P_OFF + h * SM::P_BYTES;
       for (int j = 0; j < n; ++j) {
@@ -684,7 +731,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
         }
         if (item.causal >= 0) {  // tokens after this row's own position
           const int pos0 = (item.sb_begin + j) * 64;
-          const int lim = item.causal + row / gq - pos0;  // last visible token in this tile
+          const int lim = own_pos - pos0;  // last visible token in this tile
           if (lim < 63) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
