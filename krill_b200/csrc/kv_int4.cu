@@ -46,8 +46,11 @@ __device__ __forceinline__ float sane4(float x) {
 }
 
 // Quantizes this lane's 16 elements (8 packed words); the LPG lanes of a group
-// are consecutive and aligned. codes[e] in 0..15. Every lane of the warp calls
-// it.
+// are consecutive and aligned. Element e's code is the low nibble of codes[e],
+// whose other bits are those of 1.5 * 2^23 (see chunk_byte). Every lane of the
+// warp calls it. The quotients stay in [0, 15] by themselves unless z or s was
+// rounded far from the group's minimum and range (tiny values), which the
+// group's own extremes tell; only then are they clamped.
 template <int LPG, int DT>
 __device__ __forceinline__ void quant16(uint32_t (&w)[8], uint32_t (&codes)[16], uint16_t& s16, uint16_t& z16) {
   using P = Pk<DT>;
@@ -90,26 +93,41 @@ __device__ __forceinline__ void quant16(uint32_t (&w)[8], uint32_t (&codes)[16],
   const __half hs = __float2half_rn(__fdiv_rn(mx - mn, 15.0f)), hz = __float2half_rn(mn);
   const float s = __half2float(hs), z = __half2float(hz);
   const float r = s > 0.0f ? __frcp_rn(s) : 0.0f;
+  const float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to nearest even
+  const F2 s2 = f2(-s, -s), r2 = f2(r, r), z2 = f2(-z, -z), round2 = f2(kRound, kRound);
+  auto quotient = [&](float a, float b) {
+    const F2 t = f2_add(f2(a, b), z2);
+    const F2 q = f2_mul(t, r2);
+    return f2_fma(f2_fma(q, s2, t), r2, q);
+  };
+  const F2 ends = quotient(mn, mx);
+  const bool inside = f2_lo(ends) > -0.5f && f2_hi(ends) < 15.5f;
+  if (__all_sync(0xffffffffu, inside)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 x = P::f(w[i]);
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = P::f(w[i]);
+      const F2 k = f2_add(quotient(x.x, x.y), round2);
+      codes[2 * i] = __float_as_uint(f2_lo(k));
+      codes[2 * i + 1] = __float_as_uint(f2_hi(k));
+    }
+  } else {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float t = (e ? x.y : x.x) - z;
-      float q = t * r;
-      q = fmaf(fmaf(-q, s, t), r, q);
-      q = fminf(fmaxf(q, 0.0f), 15.0f);
-      codes[2 * i + e] = __float_as_uint(q + 12582912.0f) & 15u;  // 1.5 * 2^23: rounds to nearest even
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = P::f(w[i]);
+      const F2 q = quotient(x.x, x.y);
+      codes[2 * i] = __float_as_uint(fminf(fmaxf(f2_lo(q), 0.0f), 15.0f) + kRound);
+      codes[2 * i + 1] = __float_as_uint(fminf(fmaxf(f2_hi(q), 0.0f), 15.0f) + kRound);
     }
   }
   s16 = __half_as_ushort(hs);
   z16 = __half_as_ushort(hz);
 }
 
-// Byte j of this lane's chunk (see q4_kbyte / q4_vbyte).
+// Byte j of this lane's chunk (see q4_kbyte / q4_vbyte), from codes whose bits
+// 4 to 7 are zero.
 __device__ __forceinline__ uint8_t chunk_byte(const uint32_t (&codes)[16], bool is_k, int j) {
-  return is_k ? (uint8_t)(codes[q4_elem(true, j)] | (codes[q4_elem(true, j) + q4_step(true)] << 4))
-              : (uint8_t)(codes[q4_elem(false, j)] | (codes[q4_elem(false, j) + q4_step(false)] << 4));
+  return is_k ? (uint8_t)(codes[q4_elem(true, j)] + 16u * codes[q4_elem(true, j) + q4_step(true)])
+              : (uint8_t)(codes[q4_elem(false, j)] + 16u * codes[q4_elem(false, j) + q4_step(false)]);
 }
 
 __device__ __forceinline__ void load16(const void* src, int64_t elem, uint32_t (&w)[8]) {
@@ -193,6 +211,48 @@ __global__ void __launch_bounds__(256) append4_kernel(uint8_t* __restrict__ pool
   }
 }
 
+// One thread's rows of a sub-block's K or V: chunk c of the tokens t0, t0 +
+// 4096 / D, ... (PER of them), those outside [t_lo, t_hi) as zeros.
+template <int D, int PER>
+__device__ __forceinline__ void tile_fetch(const void* src, int64_t row0, int c, int t0, int t_lo, int t_hi,
+                                           uint32_t (&w)[PER][8]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = t0 + i * (4096 / D);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[i][e] = 0u;
+    if (t >= t_lo && t < t_hi) load16(src, (row0 + t) * D + 16 * c, w[i]);
+  }
+}
+// Quantizes them into the sub-block at `to` (shared or global); true when a
+// scale is 64 or more.
+template <int D, int G, int DT, int PER, bool K>
+__device__ __forceinline__ bool tile_quantize(uint32_t (&w)[PER][8], int64_t cs, int c, int t0, int t_lo, int t_hi,
+                                              const RopeTable& rope, uint8_t* to) {
+  constexpr int LPG = G / 16, NG = D / G, a = K ? 0 : 2;
+  bool large = false;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = t0 + i * (4096 / D);
+    const bool live = t >= t_lo && t < t_hi;
+    if (K && rope.cos) rope16<D, DT>(w[i], c, cs + t, rope, live);
+    uint32_t codes[16];
+    uint16_t s16, z16;
+    quant16<LPG, DT>(w[i], codes, s16, z16);
+    if (!live) continue;
+    uint8_t* at = to + (K ? q4_kbyte(D, t, c, 0) : q4_vbyte(D, NG, t, c, 0));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) at[K ? (j >> 1) * 4 + (j & 1) * 2 : j * 64] = chunk_byte(codes, K, j);
+    if (c % LPG == 0) {
+      const int gi = c / LPG;
+      *reinterpret_cast<uint16_t*>(to + q4_meta(D, NG, a, gi, t)) = s16;
+      *reinterpret_cast<uint16_t*>(to + q4_meta(D, NG, a + 1, gi, t)) = z16;
+      large |= s16 >= 0x5400u;
+    }
+  }
+  return large;
+}
+
 // Appends of many tokens (prompts): one CTA per (layer, sequence, kv head,
 // touched sub-block). A sub-block that the call covers whole is built in shared
 // memory and leaves with 16-byte stores; one that it covers in part gets byte
@@ -206,8 +266,8 @@ __global__ void __launch_bounds__(256) append4_tile_kernel(uint8_t* __restrict__
                                                            const void* __restrict__ v,
                                                            int* __restrict__ large_scale, RopeTable rope) {
   asm volatile("griddepcontrol.launch_dependents;");  // as in append_quantize_kernel
-  constexpr int LPT = D / 16, LPG = G / 16, NG = D / G, T = kSub4;
-  constexpr int SB = T * (D + 8 * NG), ITEMS = 2 * T * LPT;
+  constexpr int LPT = D / 16, NG = D / G, T = kSub4;
+  constexpr int SB = T * (D + 8 * NG);
   __shared__ __align__(16) uint8_t img[SB];
   uint32_t b = blockIdx.x;
   const int ch = (int)(b % (uint32_t)n_chunks);
@@ -226,30 +286,15 @@ __global__ void __launch_bounds__(256) append4_tile_kernel(uint8_t* __restrict__
   const int64_t row0 = (ls * geom.Hkv + h) * n_new + (cs - p0);  // input row of token t: row0 + t
   const bool whole = t_lo == 0 && t_hi == T;
   bool large = false;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < ITEMS; i += 256) {
-    const int c = i % LPT, t = (i / LPT) % T;
-    const bool is_k = i < ITEMS / 2, live = t >= t_lo && t < t_hi;
-    uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-    if (live) load16(is_k ? k : v, (row0 + t) * D + 16 * c, w);
-    if (rope.cos) rope16<D, DT>(w, c, cs + t, rope, live && is_k);
-    uint32_t codes[16];
-    uint16_t s16, z16;
-    quant16<LPG, DT>(w, codes, s16, z16);
-    if (!live) continue;
-    auto put = [&](uint8_t* to) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) to[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, NG, t, c, j)] = chunk_byte(codes, is_k, j);
-      if (c % LPG == 0) {
-        const int gi = c / LPG, a = is_k ? 0 : 2;
-        *reinterpret_cast<uint16_t*>(to + q4_meta(D, NG, a, gi, t)) = s16;
-        *reinterpret_cast<uint16_t*>(to + q4_meta(D, NG, a + 1, gi, t)) = z16;
-        large |= s16 >= 0x5400u;
-      }
-    };
-    if (whole) put(img);
-    else put(sb);
-  }
+  // all of K's loads, then V's while K is quantized
+  constexpr int PER = T * LPT / 256;  // rounds of K (and of V) items
+  uint32_t wk[PER][8], wv[PER][8];
+  const int c = threadIdx.x % LPT, t0 = threadIdx.x / LPT;
+  tile_fetch<D, PER>(k, row0, c, t0, t_lo, t_hi, wk);
+  tile_fetch<D, PER>(v, row0, c, t0, t_lo, t_hi, wv);
+  uint8_t* to = whole ? img : sb;
+  large |= tile_quantize<D, G, DT, PER, true>(wk, cs, c, t0, t_lo, t_hi, rope, to);
+  large |= tile_quantize<D, G, DT, PER, false>(wv, cs, c, t0, t_lo, t_hi, rope, to);
   if (large) atomicOr(large_scale, 1);
   if (!whole) return;
   __syncthreads();
@@ -290,19 +335,17 @@ __device__ __forceinline__ void store16(void* out, int dtype, int64_t elem, cons
   p[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// Rows [start, start + n) of every (layer, sequence) of the call, dequantized,
-// in the layout that an append takes: [layers][seqs][Hkv][n][D]. One CTA per
-// (layer, sequence, kv head, touched sub-block), which it brings into shared
-// memory with 16-byte loads.
-template <int FMT>
-__global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t* __restrict__ pool, Geom geom,
-                                                        const int32_t* __restrict__ bt, int bt_stride,
-                                                        const int64_t* __restrict__ starts, int layer_begin,
-                                                        int n_seqs, int64_t n, int n_chunks, void* keys,
-                                                        void* values, int dtype) {
-  extern __shared__ __align__(16) uint8_t img[];
-  const int D = geom.D, NG = geom.NG, LPT = D / 16, T = geom.subt;
-  uint32_t b = blockIdx.x;
+// Where the rows [starts[si], + n) of a read lie: sub-block ch of those that
+// row range touches in (layer, sequence, kv head) of CTA b; false: none.
+struct ReadAt {
+  const uint8_t* sb;
+  int64_t row0;  // output row of the sub-block's token 0
+  int t_lo, t_hi;
+};
+__device__ __forceinline__ bool read_at(const uint8_t* pool, const Geom& geom, const int32_t* bt, int bt_stride,
+                                        const int64_t* starts, int layer_begin, int n_seqs, int64_t n, int n_chunks,
+                                        uint32_t b, ReadAt& at) {
+  const int T = geom.subt;
   const int ch = (int)(b % (uint32_t)n_chunks);
   b /= (uint32_t)n_chunks;
   const int h = (int)(b % (uint32_t)geom.Hkv);
@@ -310,42 +353,143 @@ __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t* __restric
   const int si = (int)(ls % n_seqs), layer = layer_begin + (int)(ls / n_seqs);
   const int64_t p0 = starts[si];
   const int64_t cs = p0 - p0 % T + (int64_t)ch * T;
-  const int t_lo = (int)max((int64_t)0, p0 - cs), t_hi = (int)min((int64_t)T, p0 + n - cs);
-  if (t_lo >= t_hi) return;
+  at.t_lo = (int)max((int64_t)0, p0 - cs);
+  at.t_hi = (int)min((int64_t)T, p0 + n - cs);
+  if (at.t_lo >= at.t_hi) return false;
   int64_t bi = cs / kBlockTokens;
   if (geom.ring > 0) bi %= geom.ring;
-  const uint8_t* sb = pool +
-                      (((int64_t)bt[(int64_t)si * bt_stride + bi] * geom.L + layer) * geom.Hkv + h) * geom.page_bytes +
-                      (cs % kBlockTokens) / T * geom.sb_bytes;
-  for (int i = threadIdx.x; i < (int)(geom.sb_bytes / 16); i += 256)
-    reinterpret_cast<uint4*>(img)[i] = reinterpret_cast<const uint4*>(sb)[i];
+  at.sb = pool + (((int64_t)bt[(int64_t)si * bt_stride + bi] * geom.L + layer) * geom.Hkv + h) * geom.page_bytes +
+          (cs % kBlockTokens) / T * geom.sb_bytes;
+  at.row0 = (ls * geom.Hkv + h) * n + (cs - p0);
+  return true;
+}
+
+// Rows of a 4-bit pool, dequantized, in the layout that an append takes:
+// [layers][seqs][Hkv][n][D]. One CTA per (layer, sequence, kv head, touched
+// sub-block). A thread takes four consecutive tokens (one tile row pair's) of
+// 16 elements: of K two 16-byte words, of V eight 4-byte words of the image in
+// shared memory, whose V codes are spread by 16 bytes per 512 against bank
+// conflicts. Its eight (K) lanes along D write 256 consecutive bytes a row.
+template <int D, int G>
+__global__ void __launch_bounds__(256) read_rows4_kernel(const uint8_t* __restrict__ pool, Geom geom,
+                                                         const int32_t* __restrict__ bt, int bt_stride,
+                                                         const int64_t* __restrict__ starts, int layer_begin,
+                                                         int n_seqs, int64_t n, int n_chunks, void* keys,
+                                                         void* values, int dtype) {
+  constexpr int LPT = D / 16, NG = D / G, HALF = q4_half(D, NG), CODES = 32 * D;
+  __shared__ __align__(16) uint8_t img[2 * HALF + CODES / 32];
+  ReadAt at;
+  if (!read_at(pool, geom, bt, bt_stride, starts, layer_begin, n_seqs, n, n_chunks, blockIdx.x, at)) return;
+  // image: K half, V scales and zeros, V codes (spread)
+  constexpr int VMETA = HALF, VCODES = HALF + 256 * NG;
+  for (int i = threadIdx.x; i < 2 * HALF / 16; i += 256) {
+    const int off = 16 * i;
+    int to = off;
+    if (off >= HALF + CODES) to = VMETA + off - HALF - CODES;
+    else if (off >= HALF) to = VCODES + (off - HALF) + ((off - HALF) >> 9) * 16;
+    *reinterpret_cast<uint4*>(img + to) = __ldg(reinterpret_cast<const uint4*>(at.sb) + i);
+  }
   __syncthreads();
-  const int64_t row0 = (ls * geom.Hkv + h) * n + (cs - p0);
-  const int span = (t_hi - t_lo) * LPT;
+  // 16 items of four tokens: tile u, rows 2 tig and 2 tig + 1 (both halves)
+  for (int i = threadIdx.x; i < 2 * 16 * LPT; i += 256) {
+    const bool is_k = i < 16 * LPT;
+    const int c = i % LPT, u = i / LPT % 4, tig = i / (4 * LPT) % 4, gi = 16 * c / G;
+    const int t = 16 * tig + 4 * u;  // tokens t + 2 hi + h
+    if (t + 4 <= at.t_lo || t >= at.t_hi) continue;
+    void* out = is_k ? keys : values;
+    if (!out) continue;
+    const uint8_t* meta = is_k ? img + CODES : img + VMETA;
+    float s[2][2], z[2][2];  // [h][hi]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 ss = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(meta + gi * 128 + (2 * tig + h) * 16 + 4 * u)));
+      const float2 zz =
+          __half22float2(u2h(*reinterpret_cast<const uint32_t*>(meta + (NG + gi) * 128 + (2 * tig + h) * 16 + 4 * u)));
+      s[h][0] = ss.x; s[h][1] = ss.y;
+      z[h][0] = zz.x; z[h][1] = zz.y;
+    }
+    // code words: of V word j holds the codes of elements j, j + 8 of the four
+    // tokens; of K the words of row h hold those of its two tokens
+    uint32_t w[2][4];
+    if (is_k) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 x = *reinterpret_cast<const uint4*>(img + ((u * (D / 64) + (c >> 2)) * 32 + (2 * tig + h) * 4 + (c & 3)) * 16);
+        w[h][0] = x.x; w[h][1] = x.y; w[h][2] = x.z; w[h][3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        w[j >> 2][j & 3] = *reinterpret_cast<const uint32_t*>(img + VCODES + c * 528 + (j * 4 + tig) * 16 + 4 * u);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const int tok = t + 2 * hi + h;
+        if (tok < at.t_lo || tok >= at.t_hi) continue;
+        float x[16];
+        if (is_k) {  // row h: word k, halves d = 4k, 4k + 1 (low nibbles), + 2, + 3 (high)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int nib = 0; nib < 2; ++nib) {
+              const uint32_t v = ((w[h][k] >> (8 * hi + 4 * nib)) & 0x000f000fu) | 0x64006400u;
+              const float2 f = __half22float2(__hsub2_rn(u2h(v), u2h(0x64006400u)));
+              x[4 * k + 2 * nib] = f.x;
+              x[4 * k + 2 * nib + 1] = f.y;
+            }
+        } else {  // half h of word j: byte hi, element j (low nibble) and j + 8
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t b = w[j >> 2][j & 3] >> (16 * h + 8 * hi);
+            const uint32_t v = (b & 0xfu) | ((b & 0xf0u) << 12) | 0x64006400u;
+            const float2 f = __half22float2(__hsub2_rn(u2h(v), u2h(0x64006400u)));
+            x[j] = f.x;
+            x[j + 8] = f.y;
+          }
+        }
+        const F2 s2 = f2(s[h][hi], s[h][hi]), z2 = f2(z[h][hi], z[h][hi]);
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const F2 y = f2_fma(f2(x[e], x[e + 1]), s2, z2);
+          x[e] = f2_lo(y);
+          x[e + 1] = f2_hi(y);
+        }
+        store16(out, dtype, (at.row0 + tok) * D + 16 * c, x);
+      }
+  }
+}
+
+// The same of an int8 pool.
+__global__ void __launch_bounds__(256) read_rows8_kernel(const uint8_t* __restrict__ pool, Geom geom,
+                                                         const int32_t* __restrict__ bt, int bt_stride,
+                                                         const int64_t* __restrict__ starts, int layer_begin,
+                                                         int n_seqs, int64_t n, int n_chunks, void* keys,
+                                                         void* values, int dtype) {
+  extern __shared__ __align__(16) uint8_t img8[];
+  const int D = geom.D, NG = geom.NG, LPT = D / 16;
+  ReadAt at;
+  if (!read_at(pool, geom, bt, bt_stride, starts, layer_begin, n_seqs, n, n_chunks, blockIdx.x, at)) return;
+  for (int i = threadIdx.x; i < (int)(geom.sb_bytes / 16); i += 256)
+    reinterpret_cast<uint4*>(img8)[i] = reinterpret_cast<const uint4*>(at.sb)[i];
+  __syncthreads();
+  const int span = (at.t_hi - at.t_lo) * LPT;
   for (int i = threadIdx.x; i < 2 * span; i += 256) {
     const bool is_k = i < span;
     const int j = is_k ? i : i - span;
-    const int c = j % LPT, t = t_lo + j / LPT, gi = 16 * c / geom.G, a = is_k ? 0 : 2;
+    const int c = j % LPT, t = at.t_lo + j / LPT, gi = 16 * c / geom.G, a = is_k ? 0 : 2;
     void* out = is_k ? keys : values;
     if (!out) continue;
+    const __half s = *reinterpret_cast<const __half*>(img8 + sb_meta(D, NG, a, gi, t));
+    const __half z = *reinterpret_cast<const __half*>(img8 + sb_meta(D, NG, a + 1, gi, t));
     float x[16];
-    if (FMT == kFmtInt4) {
-      uint8_t codes[16];
-      unpack_chunk(img, D, NG, t, c, is_k, codes);
-      const float s = __half2float(*reinterpret_cast<const __half*>(img + q4_meta(D, NG, a, gi, t)));
-      const float z = __half2float(*reinterpret_cast<const __half*>(img + q4_meta(D, NG, a + 1, gi, t)));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = fmaf((float)codes[e], s, z);
-    } else {
-      const __half s = *reinterpret_cast<const __half*>(img + sb_meta(D, NG, a, gi, t));
-      const __half z = *reinterpret_cast<const __half*>(img + sb_meta(D, NG, a + 1, gi, t));
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint8_t code = img[is_k ? sb_kcode(D, t, 16 * c + e) : sb_vcode(D, t, 16 * c + e)];
-        x[e] = __half2float(__hadd_rn(__hmul_rn(__ushort2half_rn(code), s), z));
-      }
+    for (int e = 0; e < 16; ++e) {
+      const uint8_t code = img8[is_k ? sb_kcode(D, t, 16 * c + e) : sb_vcode(D, t, 16 * c + e)];
+      x[e] = __half2float(__hadd_rn(__hmul_rn(__ushort2half_rn(code), s), z));
     }
-    store16(out, dtype, (row0 + t) * D + 16 * c, x);
+    store16(out, dtype, (at.row0 + t) * D + 16 * c, x);
   }
 }
 
@@ -479,13 +623,20 @@ cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const int32_t* 
   const int64_t n_chunks = (n + g.subt - 1) / g.subt + 1;
   const int64_t blocks = (int64_t)layer_count * n_seqs * g.Hkv * n_chunks;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  const size_t smem = (size_t)g.sb_bytes;
-  if (g.fmt == kFmtInt4)
-    read_rows_kernel<kFmtInt4><<<(unsigned)blocks, 256, smem, stream>>>(pool, g, d_bt, bt_stride, d_starts, layer_begin,
-                                                                        n_seqs, n, (int)n_chunks, keys, values, dtype);
-  else
-    read_rows_kernel<kFmtInt8><<<(unsigned)blocks, 256, smem, stream>>>(pool, g, d_bt, bt_stride, d_starts, layer_begin,
-                                                                        n_seqs, n, (int)n_chunks, keys, values, dtype);
+#define KRILL_READ4(DD, GG)                                                                                \
+  if (g.fmt == kFmtInt4 && g.D == DD && g.G == GG)                                                         \
+    read_rows4_kernel<DD, GG><<<(unsigned)blocks, 256, 0, stream>>>(pool, g, d_bt, bt_stride, d_starts,    \
+                                                                    layer_begin, n_seqs, n, (int)n_chunks, \
+                                                                    keys, values, dtype);
+  KRILL_READ4(64, 64)
+  KRILL_READ4(128, 64)
+  KRILL_READ4(128, 128)
+  KRILL_READ4(256, 64)
+  KRILL_READ4(256, 256)
+#undef KRILL_READ4
+  if (g.fmt != kFmtInt4)
+    read_rows8_kernel<<<(unsigned)blocks, 256, (size_t)g.sb_bytes, stream>>>(
+        pool, g, d_bt, bt_stride, d_starts, layer_begin, n_seqs, n, (int)n_chunks, keys, values, dtype);
   return cudaGetLastError();
 }
 
