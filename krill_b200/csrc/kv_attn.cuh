@@ -554,6 +554,12 @@ __device__ __forceinline__ void set_q4(TCState<D>& st, Q4State<NG>& x, const QRa
   x.zb[1] = h2u(__halves2half2(h2, __ushort_as_half(0)));
 }
 
+// to[0..1] += a[0..1] * b
+__device__ __forceinline__ void f2_fma_to(float* to, const float* a, F2 b) {
+  const F2 y = f2_fma(f2(a[0], a[1]), b, f2(to[0], to[1]));
+  to[0] = f2_lo(y);
+  to[1] = f2_hi(y);
+}
 __device__ __forceinline__ uint32_t q4_word(const uint4& w, int u) {
   return u == 0 ? w.x : u == 1 ? w.y : u == 2 ? w.z : w.w;
 }
@@ -622,9 +628,7 @@ __device__ __forceinline__ void q4_scores(const uint8_t* __restrict__ sb, TCStat
         const float2 ks = q4_pair(ksw, u0 + i);
 #pragma unroll
         for (int q = 0; q < QT; ++q)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            s[q][u0 + i][c] = fmaf(acc[q][i][c], c < 2 ? ks.x : ks.y, s[q][u0 + i][c]);
+          for (int c = 0; c < 4; c += 2) f2_fma_to(s[q][u0 + i] + c, acc[q][i] + c, c < 2 ? f2(ks.x, ks.x) : f2(ks.y, ks.y));
       }
     }
   }
@@ -667,21 +671,21 @@ __device__ __forceinline__ void q4_softmax(TCState<D> (&st)[QT], const Q4State<N
     al[q][1] = ex2_ftz(st[q].m[1] - b1);
     st[q].m[0] = mn0;
     st[q].m[1] = mn1;
-    const float e0 = bias - b0, e1 = bias - b1;
-    float ps0 = 0.f, ps1 = 0.f;
+    const F2 e = f2(bias - b0, bias - b1), cs = f2(x[q].cs[0], x[q].cs[1]);
+    F2 ps = f2(0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      s[q][u][0] = ex2_ftz(fmaf(s[q][u][0], x[q].cs[0], e0));
-      s[q][u][1] = ex2_ftz(fmaf(s[q][u][1], x[q].cs[1], e1));
-      s[q][u][2] = ex2_ftz(fmaf(s[q][u][2], x[q].cs[0], e0));
-      s[q][u][3] = ex2_ftz(fmaf(s[q][u][3], x[q].cs[1], e1));
-      ps0 += s[q][u][0] + s[q][u][2];
-      ps1 += s[q][u][1] + s[q][u][3];
-      ph[q][u][0] = f2h2(s[q][u][0], s[q][u][1]);
-      ph[q][u][1] = f2h2(s[q][u][2], s[q][u][3]);
-    }
-    st[q].l[0] = st[q].l[0] * al[q][0] + ps0;
-    st[q].l[1] = st[q].l[1] * al[q][1] + ps1;
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        const F2 y = f2_fma(f2(s[q][u][c], s[q][u][c + 1]), cs, e);
+        s[q][u][c] = ex2_ftz(f2_lo(y));
+        s[q][u][c + 1] = ex2_ftz(f2_hi(y));
+        ps = f2_add(ps, f2(s[q][u][c], s[q][u][c + 1]));
+        ph[q][u][c / 2] = f2h2(s[q][u][c], s[q][u][c + 1]);
+      }
+    ps = f2_fma(f2(st[q].l[0], st[q].l[1]), f2(al[q][0], al[q][1]), ps);
+    st[q].l[0] = f2_lo(ps);
+    st[q].l[1] = f2_hi(ps);
   }
 
 }
@@ -712,19 +716,20 @@ __device__ __forceinline__ void q4_weights(const uint8_t* __restrict__ vb, Q4Sta
     }
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-      float zs0 = 0.f, zs1 = 0.f, one[4] = {0.f, 0.f, 0.f, 0.f};
+      F2 zs = f2(0.f, 0.f);
+      float one[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const uint32_t vs = q4_word(vsw, u);
         const float2 z = __half22float2(__hfma2(u2h(0x47804780u), u2h(vs), u2h(q4_word(vzw, u))));  // z + 7.5 s
-        zs0 = fmaf(s[q][u][0], z.x, fmaf(s[q][u][2], z.y, zs0));
-        zs1 = fmaf(s[q][u][1], z.x, fmaf(s[q][u][3], z.y, zs1));
+        zs = f2_fma(f2(s[q][u][0], s[q][u][1]), f2(z.x, z.x), zs);
+        zs = f2_fma(f2(s[q][u][2], s[q][u][3]), f2(z.y, z.y), zs);
         pb[q][g][u][0] = movm_trans(h2u(__hmul2(u2h(ph[q][u][0]), u2h(__byte_perm(vs, 0, 0x1010)))));
         pb[q][g][u][1] = movm_trans(h2u(__hmul2(u2h(ph[q][u][1]), u2h(__byte_perm(vs, 0, 0x3232)))));
         mma16816(one, 0x3b803b80u, 0x3b803b80u, 0x3b803b80u, 0x3b803b80u, pb[q][g][u][0], pb[q][g][u][1]);  // 7.5 / 8
       }
-      x[q].zs[0][g] = fmaf(x[q].zs[0][g], al[q][0], zs0 - one[0]);
-      x[q].zs[1][g] = fmaf(x[q].zs[1][g], al[q][1], zs1 - one[1]);
+      x[q].zs[0][g] = fmaf(x[q].zs[0][g], al[q][0], f2_lo(zs) - one[0]);
+      x[q].zs[1][g] = fmaf(x[q].zs[1][g], al[q][1], f2_hi(zs) - one[1]);
     }
   }
 }
@@ -758,9 +763,12 @@ __device__ __forceinline__ void q4_output(const uint8_t* __restrict__ vb, TCStat
     for (int q = 0; q < QT; ++q)
 #pragma unroll
       for (int i = 0; i < ILV; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          st[q].o[mt0 + i][c] = fmaf(st[q].o[mt0 + i][c], al[q][c & 1], acc[q][i][c]);
+        for (int c = 0; c < 4; c += 2) {
+          const F2 y = f2_fma(f2(st[q].o[mt0 + i][c], st[q].o[mt0 + i][c + 1]), f2(al[q][0], al[q][1]),
+                              f2(acc[q][i][c], acc[q][i][c + 1]));
+          st[q].o[mt0 + i][c] = f2_lo(y);
+          st[q].o[mt0 + i][c + 1] = f2_hi(y);
+        }
   }
 }
 
@@ -795,10 +803,11 @@ struct AttnSmem {
   static constexpr int BAR_OFF = STAGE_BYTES;                 // 2*NSTAGE u64
   static constexpr int NV = D / 16 * 4 + 4;                   // per-lane state floats
   static constexpr int CB_OFF = BAR_OFF + 2 * NSTAGE * 8;     // [NCW - NCW/R][NV][32] f32
-  static constexpr int CB_BYTES = R > 1 ? (NCW - NCW / R) * NV * 32 * 4 : 0;
+  static constexpr int CB_BYTES = R == 1 ? 0 : (NCW - (FMT == kFmtInt4 && R >= 4 ? 0 : NCW / R)) * NV * 32 * 4;
   static constexpr int TAG_OFF = CB_OFF + CB_BYTES;           // [NSTAGE] u32 stage tags
   static constexpr int MISC_OFF = TAG_OFF + ((NSTAGE * 4 + 15) / 16) * 16;  // abort flag
-  static constexpr int TOTAL = MISC_OFF + 16;
+  static constexpr int LAST_OFF = MISC_OFF + 16;  // [8] per head: its piece arrived last (int4)
+  static constexpr int TOTAL = LAST_OFF + (FMT == kFmtInt4 ? 32 : 0);
 };
 
 // Number of stages that fit next to the rest of the shared memory.
@@ -808,6 +817,59 @@ constexpr int stages_for() {
   constexpr int most = FMT == kFmtInt4 ? 24 : 16;
   constexpr int n = (232448 - fixed - 2 * 8 * most - (FMT == kFmtInt4 ? 4 * most : 0)) / AttnSmem<D, NG, NCW, R, 0, FMT>::SB;
   return n > most ? most : n;
+}
+
+// Column hq of a split unit's kv head h from its n_split partial records, by
+// one warp: lane i holds the max and normalizer of record i (32 at a time), the
+// lanes together one row of D outputs, and the records' rows are summed in
+// record order, eight of them in flight. Read through L2: other CTAs of the
+// same launch may have written them.
+template <int D>
+__device__ __forceinline__ void combine_row(const AttnParams& p, const AttnUnit& un, int h, int hq, int lane) {
+  constexpr int V = D < 128 ? 2 : 4, EPT = D / (32 * V);  // EPT vectors of V floats per lane
+  using Vec = typename std::conditional<V == 4, float4, float2>::type;
+  const float* base = p.partials + ((int64_t)un.first_split * p.Hkv + h) * partial_floats(D);
+  const int64_t stride = (int64_t)p.Hkv * partial_floats(D);
+  const int n = un.n_split;
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(base + i * stride + hq));
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float Ls = 0.f, Os[EPT][V];
+#pragma unroll
+  for (int e = 0; e < EPT; ++e)
+#pragma unroll
+    for (int c = 0; c < V; ++c) Os[e][c] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane, m = min(32, n - i0);
+    const float mi = i < n ? __ldcg(base + i * stride + hq) : -INFINITY;
+    const float li = i < n ? __ldcg(base + i * stride + 8 + hq) : 0.f;
+    const float wi = mi == -INFINITY ? 0.f : exp2f(mi - M);
+    const float* o = base + i0 * stride + 16 + hq * D + lane * V;
+#pragma unroll 8
+    for (int k = 0; k < m; ++k) {
+      Vec x[EPT];
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) x[e] = __ldcg(reinterpret_cast<const Vec*>(o + k * stride + e * 32 * V));
+      const float mk = __shfl_sync(0xffffffffu, mi, k);
+      const float lk = __shfl_sync(0xffffffffu, li, k), wk = __shfl_sync(0xffffffffu, wi, k);
+      Ls += (mk == -INFINITY) ? 0.f : lk * wk;
+#pragma unroll
+      for (int e = 0; e < EPT; ++e)
+#pragma unroll
+        for (int c = 0; c < V; ++c) {  // (an empty record's O may be anything)
+          const float oi = reinterpret_cast<const float*>(&x[e])[c];
+          Os[e][c] = (mk != -INFINITY) ? Os[e][c] + oi * wk : Os[e][c];
+        }
+    }
+  }
+  const float inv = 1.f / Ls;
+  const int64_t orow =
+      ((int64_t)un.qo_row * p.Hq + (int64_t)h * p.g) * D + col_off(hq, p.g, (int64_t)p.Hq * D, D);
+#pragma unroll
+  for (int e = 0; e < EPT; ++e)
+#pragma unroll
+    for (int c = 0; c < V; ++c) store_out(p.out, p.out_dtype, orow + (e * 32 + lane) * V + c, Os[e][c] * inv);
 }
 
 // Merge a split unit's n_split partial records for kv head h into the output,
@@ -1003,65 +1065,19 @@ __device__ __forceinline__ void finish_head(const AttnParams& p, TCState<D>& st,
 }
 
 // Merge the partial records of split units: one warp per (split unit, kv head,
-// column of the query tile). Lane i of the warp holds the max and normalizer of
-// record i (32 at a time), the lanes together one row of D outputs, and the
-// records' rows are summed in record order, eight of them in flight. Reads
-// bound it: one CTA per (unit, kv head) whose 128 threads walked all the
+// column of the query tile). Reads bound it: one CTA per (unit, kv head) whose 128 threads walked all the
 // columns took 106 us for 12 x 2 x 4 (unit, head) pairs of 32 records at
 // head_dim 128 (12.8 MB).
 constexpr int kCombineWarps = 4;
 template <int D>
 __global__ void __launch_bounds__(32 * kCombineWarps) attn_combine_kernel(AttnParams p) {
-  constexpr int V = D < 128 ? 2 : 4, EPT = D / (32 * V);  // EPT vectors of V floats per lane
-  using Vec = typename std::conditional<V == 4, float4, float2>::type;
-  const int Hkv = p.Hkv, g = p.g, lane = threadIdx.x & 31;
+  const int Hkv = p.Hkv, lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
   const int hq = (int)(w % p.max_cols), h = (int)(w / p.max_cols % Hkv);
   const int64_t ui = w / p.max_cols / Hkv;
   if (ui >= p.n_split_units) return;
   const AttnUnit un = p.units[p.split_units[ui]];
-  if (hq >= unit_cols(un, g)) return;
-  const float* base = p.partials + ((int64_t)un.first_split * Hkv + h) * partial_floats(D);
-  const int64_t stride = (int64_t)Hkv * partial_floats(D);
-  const int n = un.n_split;
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, base[i * stride + hq]);
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  float Ls = 0.f, Os[EPT][V];
-#pragma unroll
-  for (int e = 0; e < EPT; ++e)
-#pragma unroll
-    for (int c = 0; c < V; ++c) Os[e][c] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const int i = i0 + lane, m = min(32, n - i0);
-    const float mi = i < n ? base[i * stride + hq] : -INFINITY;
-    const float li = i < n ? base[i * stride + 8 + hq] : 0.f;
-    const float wi = mi == -INFINITY ? 0.f : exp2f(mi - M);
-    const float* o = base + i0 * stride + 16 + hq * D + lane * V;
-#pragma unroll 8
-    for (int k = 0; k < m; ++k) {
-      Vec x[EPT];
-#pragma unroll
-      for (int e = 0; e < EPT; ++e) x[e] = *reinterpret_cast<const Vec*>(o + k * stride + e * 32 * V);
-      const float mk = __shfl_sync(0xffffffffu, mi, k);
-      const float lk = __shfl_sync(0xffffffffu, li, k), wk = __shfl_sync(0xffffffffu, wi, k);
-      Ls += (mk == -INFINITY) ? 0.f : lk * wk;
-#pragma unroll
-      for (int e = 0; e < EPT; ++e)
-#pragma unroll
-        for (int c = 0; c < V; ++c) {  // (an empty record's O may be anything)
-          const float oi = reinterpret_cast<const float*>(&x[e])[c];
-          Os[e][c] = (mk != -INFINITY) ? Os[e][c] + oi * wk : Os[e][c];
-        }
-    }
-  }
-  const float inv = 1.f / Ls;
-  const int64_t orow = ((int64_t)un.qo_row * p.Hq + (int64_t)h * g) * D + col_off(hq, g, (int64_t)p.Hq * D, D);
-#pragma unroll
-  for (int e = 0; e < EPT; ++e)
-#pragma unroll
-    for (int c = 0; c < V; ++c) store_out(p.out, p.out_dtype, orow + (e * 32 + lane) * V + c, Os[e][c] * inv);
+  if (hq < unit_cols(un, p.g)) combine_row<D>(p, un, h, hq, lane);
 }
 template <int D>
 cudaError_t run_combine(const AttnParams& p, cudaStream_t stream) {
@@ -1283,6 +1299,111 @@ __device__ __forceinline__ void attn_consume(const AttnParams& p, uint8_t* smem,
   }
 }
 
+// Finish one (item, head) with its R warps together (R >= 4): every warp leaves
+// its state in shared memory, then each takes a share of the output elements
+// and merges, normalises and stores it (or the partial record; the warps of
+// the piece that arrives last then merge the unit's records, a column each).
+// One warp doing all of it took 4 of a short item's 20 us at head_dim 256.
+template <int D, int NCW, int R, typename SM>
+__device__ __forceinline__ void finish_together(const AttnParams& p, const TCState<D>& st, float l0, float l1,
+                                                uint8_t* smem, int unit, const AttnItem& item, int h, int hr, int rr,
+                                                int lane) {
+  const int r = lane >> 2, tig = lane & 3, c0 = 2 * tig, c1 = c0 + 1;
+  float* cb = reinterpret_cast<float*>(smem + SM::CB_OFF) + (size_t)hr * R * SM::NV * 32 + lane;
+  volatile int* last_s = reinterpret_cast<volatile int*>(smem + SM::LAST_OFF) + hr;
+  auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + hr), "r"(R * 32) : "memory"); };
+  sync();  // the buffer's last readers are done
+  {
+    float* mine = cb + rr * SM::NV * 32;
+#pragma unroll
+    for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) mine[(mt * 4 + c) * 32] = st.o[mt][c];
+    mine[(D / 4 + 0) * 32] = st.m[0];
+    mine[(D / 4 + 1) * 32] = st.m[1];
+    mine[(D / 4 + 2) * 32] = l0;
+    mine[(D / 4 + 3) * 32] = l1;
+  }
+  sync();
+  const AttnUnit un = p.units[unit];
+  const int cols = unit_cols(un, p.g), n_pre = un.n_split == 1 ? un.n_pre : 0;
+  const float* rec = p.partials + ((int64_t)un.first_split * p.Hkv + h) * partial_floats(D);
+  const int64_t stride = (int64_t)p.Hkv * partial_floats(D);
+  float M0 = -INFINITY, M1 = -INFINITY, a0[R], a1[R], L0 = 0.f, L1 = 0.f;
+#pragma unroll
+  for (int w = 0; w < R; ++w) {
+    a0[w] = cb[(w * SM::NV + D / 4 + 0) * 32];
+    a1[w] = cb[(w * SM::NV + D / 4 + 1) * 32];
+    M0 = fmaxf(M0, a0[w]);
+    M1 = fmaxf(M1, a1[w]);
+  }
+  for (int i = 0; i < n_pre; ++i) {  // prefix records that the cascade kernel left
+    M0 = fmaxf(M0, rec[i * stride + c0]);
+    M1 = fmaxf(M1, rec[i * stride + c1]);
+  }
+#pragma unroll
+  for (int w = 0; w < R; ++w) {
+    a0[w] = a0[w] == -INFINITY ? 0.f : exp2f(a0[w] - M0);
+    a1[w] = a1[w] == -INFINITY ? 0.f : exp2f(a1[w] - M1);
+    L0 += cb[(w * SM::NV + D / 4 + 2) * 32] * a0[w];
+    L1 += cb[(w * SM::NV + D / 4 + 3) * 32] * a1[w];
+  }
+  // (columns past the unit's hold no prefix record: their words are read, as
+  // the buffer spans all eight, and discarded)
+  for (int i = 0; i < n_pre; ++i) {
+    const float* ri = rec + i * stride;
+    L0 += ri[c0] == -INFINITY || c0 >= cols ? 0.f : ri[8 + c0] * exp2f(ri[c0] - M0);
+    L1 += ri[c1] == -INFINITY || c1 >= cols ? 0.f : ri[8 + c1] * exp2f(ri[c1] - M1);
+  }
+  const bool split = un.n_split > 1;
+  const float i0 = 1.f / L0, i1 = 1.f / L1;
+  const int64_t row_elems = (int64_t)p.Hq * D, orow = ((int64_t)un.qo_row * p.Hq + (int64_t)h * p.g) * D;
+  const int64_t o0 = orow + col_off(c0, p.g, row_elems, D), o1 = orow + col_off(c1, p.g, row_elems, D);
+  float* part = p.partials + (((int64_t)un.first_split + item.idx) * p.Hkv + h) * partial_floats(D);
+#pragma unroll 2
+  for (int e = rr; e < D / 8; e += R) {  // row half e % 2 of row tile e / 2
+    float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < R; ++w) {
+      x0 = fmaf(cb[(w * SM::NV + 2 * e) * 32], a0[w], x0);
+      x1 = fmaf(cb[(w * SM::NV + 2 * e + 1) * 32], a1[w], x1);
+    }
+    const int d = 8 * e + r;
+    for (int i = 0; i < n_pre; ++i) {
+      const float* ri = rec + i * stride;
+      const float v0 = ri[16 + c0 * D + d], v1 = ri[16 + c1 * D + d];
+      if (ri[c0] != -INFINITY && c0 < cols) x0 = fmaf(v0, exp2f(ri[c0] - M0), x0);
+      if (ri[c1] != -INFINITY && c1 < cols) x1 = fmaf(v1, exp2f(ri[c1] - M1), x1);
+    }
+    if (split) {
+      part[16 + c0 * D + d] = x0;
+      part[16 + c1 * D + d] = x1;
+    } else {
+      if (c0 < cols) store_out(p.out, p.out_dtype, o0 + d, x0 * i0);
+      if (c1 < cols) store_out(p.out, p.out_dtype, o1 + d, x1 * i1);
+    }
+  }
+  if (!split) return;
+  if (rr == 0 && r == 0) {
+    part[c0] = M0;
+    part[c1] = M1;
+    part[8 + c0] = L0;
+    part[8 + c1] = L1;
+  }
+  if (p.split_ctr == nullptr) return;
+  __threadfence();  // this lane's stores, device-wide, before the head's count
+  sync();
+  if (rr == 0) {
+    const int last = arrive_split(p, un, h, lane) ? 1 : 0;
+    if (lane == 0) *last_s = last;
+  }
+  sync();
+  if (*last_s) {
+    __threadfence();  // the other pieces' records, before reading them
+    for (int hq = rr; hq < cols; hq += R) combine_row<D>(p, un, h, hq, lane);
+  }
+}
+
 // Consumer warps for 4-bit pools. Little is kept in registers between items
 // (the producer warp has their records and queries in the caches by then).
 template <int D, int NG, int NCW, int R, int NSTAGE, int QT, bool SEL>
@@ -1356,25 +1477,32 @@ __device__ __forceinline__ void attn_consume4(const AttnParams& p, uint8_t* smem
           l0 += __shfl_xor_sync(0xffffffffu, l0, off);
           l1 += __shfl_xor_sync(0xffffffffu, l1, off);
         }
-        merge_warps<D, NCW, R, SM>(st[q], l0, l1, smem, hr, rr, lane);
-        if (rr == 0) finish_head<D>(p, st[q], l0, l1, p.units[item.unit + q], item, h, lane);
+        if constexpr (R >= 4) {
+          finish_together<D, NCW, R, SM>(p, st[q], l0, l1, smem, item.unit, item, h, hr, rr, lane);
+        } else {  // (two warps: the other one goes on with the next item meanwhile)
+          merge_warps<D, NCW, R, SM>(st[q], l0, l1, smem, hr, rr, lane);
+          if (rr == 0) finish_head<D>(p, st[q], l0, l1, p.units[item.unit + q], item, h, lane);
+        }
       }
     }
   }
 }
 
-// Producer of 4-bit pools and of picked blocks: eight lanes issue eight
-// consecutive copies at a time. (A 4-bit sub-block is half an int8 one; issued
+// Producer of 4-bit pools and of picked blocks: W lanes issue W consecutive
+// copies at a time. (A 4-bit sub-block is half an int8 one; issued
 // by one lane, whose wait, tag, arrive and copy follow one another, the copies
 // of the batch of 32 sequences alone took 183 us where their bytes need 139.)
-// Each lane finds the source of its next copy - the picked block's index and
-// the block table entry - before it waits for the stage of the current one.
+// Sources are found 32 at a time, one per lane (the picked block's index, then
+// the block table entry: two dependent loads of a microsecond together), a
+// batch ahead of the copies.
 template <int D, int NG, int NCW, int R, int NSTAGE, int FMT, bool SEL>
 __device__ __forceinline__ void produce_wide(const AttnParams& p, uint8_t* stages, uint32_t bar_base,
                                              volatile int* cta_abort, volatile uint32_t* tags, int lane, int it0,
                                              int it1, int rounds) {
   using SG = SubGeom<D, NG, FMT>;
-  constexpr int HPR = NCW / R, SB = SG::SB, SPB = SG::SPB, W = 8;
+  // copies of a step: a third of the stages at most, so that waiting for the
+  // last of them does not hold back many that are free
+  constexpr int HPR = NCW / R, SB = SG::SB, SPB = SG::SPB, W = NSTAGE >= 20 ? 8 : NSTAGE >= 12 ? 4 : 2;
   static_assert(NSTAGE >= W, "a step's copies must not wait for one another");
   const int Hkv = p.Hkv;
   // copy i of round rd of an item: its sub-block i / HPR of head i % HPR
@@ -1390,8 +1518,8 @@ __device__ __forceinline__ void produce_wide(const AttnParams& p, uint8_t* stage
   if (it0 >= it1) return;
   AttnItem item = p.items[it0], item_n{};
   int layer = p.units[item.unit].layer, si = p.units[item.unit].si, layer_n = 0, si_n = 0;
-  const uint8_t* src = nullptr;
-  if (lane < W && lane < (item.sb_end - item.sb_begin) * HPR) src = source(item, layer, si, 0, lane);
+  const uint8_t* src = nullptr;  // of copy q + lane
+  if (lane < (item.sb_end - item.sb_begin) * HPR) src = source(item, layer, si, 0, lane);
   uint32_t J = 0;
   for (int it = it0; it < it1; ++it) {
     if (it + 1 < it1) {
@@ -1407,29 +1535,31 @@ __device__ __forceinline__ void produce_wide(const AttnParams& p, uint8_t* stage
     }
     const int total = (item.sb_end - item.sb_begin) * HPR;
     for (int rd = 0; rd < rounds; ++rd) {
-      for (int q = 0; q < total; q += W) {
+      for (int q = 0; q < total; q += 32) {
         const uint8_t* next = nullptr;
-        if (lane < W) {
-          if (q + W < total) {
-            if (q + W + lane < total) next = source(item, layer, si, rd, q + W + lane);
-          } else if (rd + 1 < rounds) {
-            if (lane < total) next = source(item, layer, si, rd + 1, lane);
-          } else if (it + 1 < it1) {
-            if (lane < (item_n.sb_end - item_n.sb_begin) * HPR) next = source(item_n, layer_n, si_n, 0, lane);
-          }
+        if (q + 32 < total) {
+          if (q + 32 + lane < total) next = source(item, layer, si, rd, q + 32 + lane);
+        } else if (rd + 1 < rounds) {
+          if (lane < total) next = source(item, layer, si, rd + 1, lane);
+        } else if (it + 1 < it1) {
+          if (lane < (item_n.sb_end - item_n.sb_begin) * HPR) next = source(item_n, layer_n, si_n, 0, lane);
         }
-        if (src != nullptr) {
-          const uint32_t Jh = J + (uint32_t)(q + lane);
-          const uint32_t stage = Jh % NSTAGE;
-          if (Jh >= (uint32_t)NSTAGE)
-            mbar_wait(bar_base + 8 * (NSTAGE + stage), ((Jh / NSTAGE) - 1) & 1, cta_abort, p.err);
-          const uint32_t full = bar_base + 8 * stage;
-          tags[stage] = Jh;  // released by the arrive below
-          mbar_expect_tx(full, SB);
-          bulk_g2s(smem_u32(stages + (size_t)stage * SB), src, SB, full);
+        for (int j = 0; j < min(32, total - q); j += W) {
+          const uint8_t* from =
+              reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (j + lane) & 31));
+          if (lane < W && q + j + lane < total) {
+            const uint32_t Jh = J + (uint32_t)(q + j + lane);
+            const uint32_t stage = Jh % NSTAGE;
+            if (Jh >= (uint32_t)NSTAGE)
+              mbar_wait(bar_base + 8 * (NSTAGE + stage), ((Jh / NSTAGE) - 1) & 1, cta_abort, p.err);
+            const uint32_t full = bar_base + 8 * stage;
+            tags[stage] = Jh;  // released by the arrive below
+            mbar_expect_tx(full, SB);
+            bulk_g2s(smem_u32(stages + (size_t)stage * SB), from, SB, full);
+          }
+          __syncwarp();
         }
         src = next;
-        __syncwarp();
       }
       J += (uint32_t)total;
     }
