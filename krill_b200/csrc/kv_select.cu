@@ -126,11 +126,11 @@ __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __r
 }
 
 constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;
-constexpr int kRegKeys = 16;             // keys a thread holds while it picks
+constexpr int kRankKeys = 256;             // most blocks that are picked by counting ranks
 constexpr uint32_t kForced = 0xffffffffu;  // above the key of every score
 
-// Order-preserving key of a score, at least 1 (equal scores, +-0 included, get
-// equal keys).
+// Order-preserving key of a score, at least 1 and below kForced (equal scores,
+// +-0 included, get equal keys).
 __device__ __forceinline__ uint32_t score_key(float x) {
   const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
   if (isnan(x)) return 1u;
@@ -145,145 +145,157 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
 }
 
 struct PickSmem {
-  uint32_t red[2][kSelWarps];          // double-buffered block reductions
-  uint32_t cnt[kRegKeys][kSelWarps];   // per key round and warp: picked-for-sure | equal << 16
+  uint32_t bins[256];
+  uint32_t lo[kSelWarps], hi[kSelWarps];
+  uint32_t gt[kSelWarps], eq[kSelWarps];  // per warp: keys above the threshold, equal to it
+  uint32_t bin, above, in_bin;
 };
 
-// Sum / min / max over the NW warps that pick (one: no barrier).
-template <int NW, typename F>
-__device__ __forceinline__ uint32_t pick_reduce(uint32_t x, PickSmem& sm, int& buf, int warp, int lane, F op) {
-  if (NW == 1) return x;
-  if (lane == 0) sm.red[buf][warp] = x;
-  __syncthreads();
-  x = sm.red[buf][0];
+// Up to 256 keys: a key is picked when fewer than `budget` keys come before it
+// (larger, or equal with a lower index), which every thread counts for its two
+// against all keys, read four at a time; the picked ones' order by ballots.
+// keys: shared memory, padded with zeros to a multiple of four.
+__device__ __forceinline__ void pick_by_rank(const uint32_t* keys, int n, int budget, int32_t* out, PickSmem& sm,
+                                             int warp, int lane) {
+  bool on[2];
+  uint32_t votes[2];
 #pragma unroll
-  for (int w = 1; w < NW; ++w) x = op(x, sm.red[buf][w]);
-  buf ^= 1;
-  return x;
+  for (int j = 0; j < 2; ++j) {
+    const int i = 64 * warp + 32 * j + lane;  // a warp's indices are consecutive
+    on[j] = false;
+    votes[j] = 0u;
+    if (64 * warp + 32 * j < n) {
+      const uint32_t k = i < n ? keys[i] : 0u;
+      int before = 0;
+#pragma unroll 4
+      for (int m = 0; m < n; m += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(keys + m);
+        before += o.x > k || (o.x == k && m < i) ? 1 : 0;
+        before += o.y > k || (o.y == k && m + 1 < i) ? 1 : 0;
+        before += o.z > k || (o.z == k && m + 2 < i) ? 1 : 0;
+        before += o.w > k || (o.w == k && m + 3 < i) ? 1 : 0;
+      }
+      on[j] = i < n && before < budget;
+      votes[j] = __ballot_sync(0xffffffffu, on[j]);
+    }
+  }
+  if (lane == 0) sm.gt[warp] = __popc(votes[0]) + __popc(votes[1]);
+  __syncthreads();
+  int at = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) at += w < warp ? (int)sm.gt[w] : 0;
+  const uint32_t below = (1u << lane) - 1u;
+  if (on[0]) out[at + __popc(votes[0] & below)] = 64 * warp + lane;
+  if (on[1]) out[at + __popc(votes[0]) + __popc(votes[1] & below)] = 64 * warp + 32 + lane;
 }
 
-// The `want` largest keys (equal ones: the first) besides the forced ones, at
-// most kRegKeys * 32 * NW of them, by bisection over the bits in which the keys
-// differ, each thread holding its keys in registers; their indices to `out` in
-// order. NW warps call it.
-template <int NW>
-__device__ __forceinline__ void pick_in_registers(const uint32_t* keys, int n, int want, int32_t* out, PickSmem& sm,
-                                                  int warp, int lane) {
-  constexpr int STEP = 32 * NW;
-  const int at = warp * 32 + lane, rounds = (n + STEP - 1) / STEP;
-  uint32_t k[kRegKeys], lo = 0xffffffffu, hi = 0u;
-  int buf = 0;
-#pragma unroll
-  for (int j = 0; j < kRegKeys; ++j) {
-    k[j] = 0u;
-    if (j < rounds) {
-      if (at + j * STEP < n) k[j] = keys[at + j * STEP];
-      if (k[j] != 0u && k[j] != kForced) {
-        lo = min(lo, k[j]);
-        hi = max(hi, k[j]);
-      }
+// Any number of keys: the threshold is found eight bits at a time, from the
+// highest bit in which the scored keys differ, by histograms over the keys that
+// share the bits found so far; usually two passes leave as many keys as are
+// still wanted. `want`: keys to pick besides the forced ones.
+__device__ __forceinline__ void pick_by_digits(const uint32_t* keys, int n, int want, int32_t* out, PickSmem& sm,
+                                               int tid, int warp, int lane) {
+  uint32_t lo = kForced, hi = 0u;
+  for (int i = tid; i < n; i += kSelThreads) {
+    const uint32_t k = keys[i];
+    if (k != kForced) {
+      lo = min(lo, k);
+      hi = max(hi, k);
     }
   }
-  lo = pick_reduce<NW>(__reduce_min_sync(0xffffffffu, lo), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return min(a, b); });
-  hi = pick_reduce<NW>(__reduce_max_sync(0xffffffffu, hi), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return max(a, b); });
-  // K: the largest threshold with at least `want` keys in [K, kForced)
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    sm.lo[warp] = lo;
+    sm.hi[warp] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    lo = min(lo, sm.lo[w]);
+    hi = max(hi, sm.hi[w]);
+  }
+  // picked: keys > K, and of those equal to K the first `need`
   uint32_t K = kForced - 1u;
-  int above = 0;
+  int need = 0;
   if (want > 0) {
-    const int top = 32 - __clz(lo ^ hi);  // bits that differ
-    K = top >= 32 ? 0u : lo >> top << top;
-    for (int bit = top - 1; bit >= 0; --bit) {
-      const uint32_t cand = K | (1u << bit);
-      uint32_t c = 0;
+    int rem = 32 - __clz(lo ^ hi);  // bits not found yet
+    uint32_t P = rem >= 32 ? 0u : lo >> rem << rem;
+    need = want;
+    bool all = false;  // every key from P on is picked
+    while (rem > 0 && !all) {
+      const int width = min(8, rem), shift = rem - width;
+      for (int i = tid; i < 256; i += kSelThreads) sm.bins[i] = 0u;
+      __syncthreads();
+      for (int i = tid; i < n; i += kSelThreads) {
+        const uint32_t k = keys[i];
+        if (k != kForced && (rem >= 32 || k >> rem == P >> rem)) atomicAdd(&sm.bins[(k >> shift) & 255u], 1u);
+      }
+      __syncthreads();
+      if (warp == 0) {  // lane l: bins 8 (31 - l) .. + 7, so that lower lanes hold larger keys
+        uint32_t c[8], sum = 0u;
 #pragma unroll
-      for (int j = 0; j < kRegKeys; ++j)
-        if (j < rounds) c += k[j] >= cand && k[j] != kForced ? 1u : 0u;
-      c = pick_reduce<NW>(__reduce_add_sync(0xffffffffu, c), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return a + b; });
-      if ((int)c >= want) K = cand;
-      if ((int)c == want) break;  // exactly the keys from K on
-    }
-    uint32_t c = 0;
+        for (int e = 0; e < 8; ++e) {
+          c[e] = sm.bins[8 * (31 - lane) + e];
+          sum += c[e];
+        }
+        uint32_t upto = sum;  // keys in this lane's bins and above
 #pragma unroll
-    for (int j = 0; j < kRegKeys; ++j)
-      if (j < rounds) c += k[j] > K && k[j] != kForced ? 1u : 0u;
-    above = (int)pick_reduce<NW>(__reduce_add_sync(0xffffffffu, c), sm, buf, warp, lane, [](uint32_t a, uint32_t b) { return a + b; });
-  }
-  const int need = want - above;  // of the keys equal to K, the first ones
-  // positions: keys above K (forced ones among them) before, and equal ones
-  uint32_t mg[kRegKeys], me[kRegKeys];
+        for (int off = 1; off < 32; off <<= 1) {
+          const uint32_t o = __shfl_up_sync(0xffffffffu, upto, off);
+          if (lane >= off) upto += o;
+        }
+        uint32_t above = upto - sum;
+        if ((int)above < need && (int)upto >= need) {  // the threshold's bin is one of this lane's
 #pragma unroll
-  for (int j = 0; j < kRegKeys; ++j)
-    if (j < rounds) {
-      mg[j] = __ballot_sync(0xffffffffu, k[j] > K);
-      me[j] = __ballot_sync(0xffffffffu, k[j] == K && K != 0u);
-      if (NW > 1 && lane == 0) sm.cnt[j][warp] = __popc(mg[j]) | (__popc(me[j]) << 16);
-    }
-  if (NW > 1) __syncthreads();
-  const uint32_t below = (1u << lane) - 1u;
-  int g0 = 0, e0 = 0;
-#pragma unroll
-  for (int j = 0; j < kRegKeys; ++j)
-    if (j < rounds) {
-      int gb = g0, eb = e0;
-      if (NW == 1) {
-        g0 += __popc(mg[j]);
-        e0 += __popc(me[j]);
-      } else {
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const uint32_t c = sm.cnt[j][w];
-          if (w < warp) {
-            gb += c & 0xffff;
-            eb += c >> 16;
+          for (int e = 7; e >= 0; --e) {
+            if ((int)above < need && (int)(above + c[e]) >= need) {
+              sm.bin = 8 * (31 - lane) + e;
+              sm.above = above;
+              sm.in_bin = c[e];
+            }
+            above += c[e];
           }
-          g0 += c & 0xffff;
-          e0 += c >> 16;
         }
       }
-      gb += __popc(mg[j] & below);
-      eb += __popc(me[j] & below);
-      const bool gt = (mg[j] >> lane) & 1u, eq = (me[j] >> lane) & 1u;
-      if (gt || (eq && eb < need)) out[gb + min(eb, need)] = at + j * STEP;
+      __syncthreads();
+      P |= sm.bin << shift;
+      need -= (int)sm.above;
+      all = (int)sm.in_bin == need;
+      rem = shift;
     }
-}
-
-// The same for any number of keys, read again in every round.
-__device__ __forceinline__ void pick_in_memory(const uint32_t* keys, int n, int budget, int32_t* out, PickSmem& sm,
-                                               int tid, int warp, int lane) {
-  int buf = 0;
-  auto add = [](uint32_t a, uint32_t b) { return a + b; };
-  auto count = [&](uint32_t from) {
-    uint32_t c = 0;
-    for (int i = tid; i < n; i += kSelThreads) c += keys[i] >= from ? 1u : 0u;
-    return (int)pick_reduce<kSelWarps>(__reduce_add_sync(0xffffffffu, c), sm, buf, warp, lane, add);
-  };
-  uint32_t K = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = K | (1u << bit);
-    if (count(cand) >= budget) K = cand;
+    K = all && P > 0u ? P - 1u : P;  // (keys are at least 1: K = 0 takes every one)
+    if (all) need = 0;
   }
-  const int need = budget - (K == kForced ? 0 : count(K + 1u));
-  int gt_before = 0, eq_before = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < n ? keys[i] : 0u;
-    const bool gt = i < n && k > K, eq = i < n && k == K;
-    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) sm.red[buf][warp] = __popc(mg) | (__popc(me) << 16);
-    __syncthreads();
-    uint32_t before = 0, total = 0;
+  // order: each warp a contiguous quarter
+  const int per = (n + kSelThreads - 1) / kSelThreads * 32, i0 = warp * per, i1 = min(n, i0 + per);
+  uint32_t ng = 0u, ne = 0u;
+  for (int i = i0; i < i1; i += 32) {
+    const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
+    ng += __popc(__ballot_sync(0xffffffffu, k > K));
+    ne += __popc(__ballot_sync(0xffffffffu, k == K && k != 0u));
+  }
+  if (lane == 0) {
+    sm.gt[warp] = ng;
+    sm.eq[warp] = ne;
+  }
+  __syncthreads();
+  int gb = 0, eb = 0;
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) {
-      if (w < warp) before += sm.red[buf][w];
-      total += sm.red[buf][w];
+  for (int w = 0; w < kSelWarps; ++w)
+    if (w < warp) {
+      gb += sm.gt[w];
+      eb += sm.eq[w];
     }
-    const uint32_t below = (1u << lane) - 1u;
-    const int gb = gt_before + (before & 0xffff) + __popc(mg & below);
-    const int eb = eq_before + (before >> 16) + __popc(me & below);
-    if (gt || (eq && eb < need)) out[gb + min(eb, need)] = i;
-    gt_before += total & 0xffff;
-    eq_before += total >> 16;
-    buf ^= 1;
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i = i0; i < i1; i += 32) {
+    const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
+    const bool gt = k > K, eq = k == K && k != 0u;
+    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+    const int g = gb + __popc(mg & below), e = eb + __popc(me & below);
+    if (gt || (eq && e < need)) out[g + min(e, need)] = i + lane;
+    gb += __popc(mg);
+    eb += __popc(me);
   }
 }
 
@@ -292,13 +304,14 @@ __device__ __forceinline__ void pick_in_memory(const uint32_t* keys, int n, int 
 // MMAs (rows = blocks, columns = query heads, K = the 2 D summary bytes; the
 // byte order along K is permuted alike on both sides, so that a lane's operand
 // is 16 consecutive bytes); the keys go to the first CTA's shared memory (or
-// to scratch, for sequences of more blocks than fit), which picks: up to 512
-// blocks in one warp without barriers, up to 2048 in four, more by reading the
-// keys again for each bit.
+// to scratch, for sequences of more blocks than fit), which picks. Latency
+// bounds it: the summaries of a warp's next 16 blocks are fetched while it
+// works on the ones before (the first while the query is rounded), their block
+// ids a step earlier.
 template <int D>
 __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
-  extern __shared__ uint32_t keys_smem[];
+  extern __shared__ __align__(16) uint32_t keys_smem[];
   __shared__ __align__(16) int8_t qa[8][2 * D];
   __shared__ float tau_s[8];
   __shared__ PickSmem sm;
@@ -316,16 +329,51 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
     return;
   }
   const int g = p.g, lo = p.first, hi = n - p.last;  // scored blocks [lo, hi)
-  // ---- the query heads in whole numbers, one warp per head ----
+  const int r = lane >> 2, tig = lane & 3;
+  constexpr int NC = 2 * D / 64;
+  const int32_t* bt = p.bt + (int64_t)si * p.bt_stride;
+  const uint8_t* base = p.pool + ((int64_t)layer * p.Hkv + h) * p.page_bytes + p.sum_off;
+  const int64_t blk_stride = (int64_t)p.L * p.Hkv * p.page_bytes;
+  const int spb_bytes = p.spb * 2 * D, step = 16 * CL * kSelWarps;
+  uint4 xa[NC], xb[NC];
+  float sa = 0.f, sb = 0.f;
+  auto block_of = [&](int i) { return __ldg(bt + min(i, hi - 1) / p.spb); };
+  auto fetch = [&](int i0, int ba, int bb) {
+    const int ra = min(i0 + r, hi - 1) % p.spb, rb = min(i0 + r + 8, hi - 1) % p.spb;
+    const uint8_t* pa = base + (int64_t)ba * blk_stride;
+    const uint8_t* pb = base + (int64_t)bb * blk_stride;
+    const uint4* wa = reinterpret_cast<const uint4*>(pa + ra * 2 * D) + tig;
+    const uint4* wb = reinterpret_cast<const uint4*>(pb + rb * 2 * D) + tig;
+    sa = __ldg(reinterpret_cast<const float*>(pa + spb_bytes) + ra);
+    sb = __ldg(reinterpret_cast<const float*>(pb + spb_bytes) + rb);
 #pragma unroll
-  for (int hq = warp; hq < 8; hq += kSelWarps) {
-    float x[D / 32], mx = 0.f;
+    for (int c = 0; c < NC; ++c) {
+      xa[c] = __ldg(wa + 4 * c);
+      xb[c] = __ldg(wb + 4 * c);
+    }
+  };
+  int i0 = lo + 16 * (rank * kSelWarps + warp);
+  int ba = block_of(i0 + r), bb = block_of(i0 + r + 8);
+  int ba_n = block_of(i0 + step + r), bb_n = block_of(i0 + step + r + 8);
+  // ---- the query heads in whole numbers, one warp per head (two rounds) ----
+  constexpr int QR = 8 / kSelWarps;
+  float x[QR][D / 32];
+#pragma unroll
+  for (int j = 0; j < QR; ++j) {
+    const int hq = warp + j * kSelWarps;
     const int64_t q0 = ((int64_t)qo_row * p.Hq + (int64_t)h * g + hq) * D;
 #pragma unroll
+    for (int i = 0; i < D / 32; ++i) x[j][i] = hq < g ? load_in(p.q, q0 + lane + 32 * i, p.q_dtype) : 0.f;
+  }
+  if (i0 < hi) fetch(i0, ba, bb);
+#pragma unroll
+  for (int j = 0; j < QR; ++j) {
+    const int hq = warp + j * kSelWarps;
+    float mx = 0.f;
+#pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      x[i] = hq < g ? load_in(p.q, q0 + lane + 32 * i, p.q_dtype) : 0.f;
-      if (!isfinite(x[i])) x[i] = 0.f;
-      mx = fmaxf(mx, fabsf(x[i]));
+      if (!isfinite(x[j][i])) x[j][i] = 0.f;
+      mx = fmaxf(mx, fabsf(x[j][i]));
     }
     // (non-negative floats order like their bits)
     mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
@@ -333,55 +381,39 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
     const float inv = tau > 0.f ? __fdiv_rn(1.0f, tau) : 0.f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      const int a = max(-127, min(127, __float2int_rn(__fmul_rn(x[i], inv))));
+      const int a = max(-127, min(127, __float2int_rn(__fmul_rn(x[j][i], inv))));
       qa[hq][lane + 32 * i] = (int8_t)a;
       qa[hq][D + lane + 32 * i] = (int8_t)abs(a);
     }
     if (lane == 0) tau_s[hq] = tau;
   }
   __syncthreads();
-  const int r = lane >> 2, tig = lane & 3;
-  constexpr int NC = 2 * D / 64;
-  uint4 bq[NC];  // column r = query head r
-#pragma unroll
-  for (int c = 0; c < NC; ++c) bq[c] = *reinterpret_cast<const uint4*>(&qa[r][64 * c + 16 * tig]);
   const float tau0 = tau_s[2 * tig], tau1 = tau_s[2 * tig + 1];
   const bool has0 = 2 * tig < g, has1 = 2 * tig + 1 < g;
   uint32_t* keys = p.scratch ? p.scratch + (int64_t)uid * p.scratch_stride
                              : cluster.map_shared_rank(keys_smem, 0);
-  const int32_t* bt = p.bt + (int64_t)si * p.bt_stride;
-  const uint8_t* base = p.pool + ((int64_t)layer * p.Hkv + h) * p.page_bytes + p.sum_off;
-  const int64_t blk_stride = (int64_t)p.L * p.Hkv * p.page_bytes;
-  const int spb_bytes = p.spb * 2 * D;
-#pragma unroll 2
-  for (int i0 = lo + 16 * (rank * kSelWarps + warp); i0 < hi; i0 += 16 * CL * kSelWarps) {
-    const int ra = min(i0 + r, hi - 1), rb = min(i0 + r + 8, hi - 1);
-    const uint8_t* pa = base + (int64_t)__ldg(bt + ra / p.spb) * blk_stride;
-    const uint8_t* pb = base + (int64_t)__ldg(bt + rb / p.spb) * blk_stride;
-    const uint4* wa = reinterpret_cast<const uint4*>(pa + (ra % p.spb) * 2 * D) + tig;
-    const uint4* wb = reinterpret_cast<const uint4*>(pb + (rb % p.spb) * 2 * D) + tig;
-    const float sa = __ldg(reinterpret_cast<const float*>(pa + spb_bytes) + ra % p.spb);
-    const float sb = __ldg(reinterpret_cast<const float*>(pb + spb_bytes) + rb % p.spb);
-    uint4 xa[NC], xb[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      xa[c] = __ldg(wa + 4 * c);
-      xb[c] = __ldg(wb + 4 * c);
-    }
+  for (; i0 < hi; i0 += step) {
     int acc[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      imma16832(acc, xa[c].x, xb[c].x, xa[c].y, xb[c].y, bq[c].x, bq[c].y);
-      imma16832(acc, xa[c].z, xb[c].z, xa[c].w, xb[c].w, bq[c].z, bq[c].w);
+    for (int c = 0; c < NC; ++c) {  // column r = query head r
+      const uint4 bq = *reinterpret_cast<const uint4*>(&qa[r][64 * c + 16 * tig]);
+      imma16832(acc, xa[c].x, xb[c].x, xa[c].y, xb[c].y, bq.x, bq.y);
+      imma16832(acc, xa[c].z, xb[c].z, xa[c].w, xb[c].w, bq.z, bq.w);
+    }
+    const float ta = sa, tb = sb;
+    if (i0 + step < hi) {
+      fetch(i0 + step, ba_n, bb_n);
+      ba_n = block_of(i0 + 2 * step + r);
+      bb_n = block_of(i0 + 2 * step + r + 8);
     }
     float va = -INFINITY, vb = -INFINITY;
     if (has0) {
-      va = __fmul_rn(__fmul_rn((float)acc[0], sa), tau0);
-      vb = __fmul_rn(__fmul_rn((float)acc[2], sb), tau0);
+      va = __fmul_rn(__fmul_rn((float)acc[0], ta), tau0);
+      vb = __fmul_rn(__fmul_rn((float)acc[2], tb), tau0);
     }
     if (has1) {
-      va = fmaxf(va, __fmul_rn(__fmul_rn((float)acc[1], sa), tau1));
-      vb = fmaxf(vb, __fmul_rn(__fmul_rn((float)acc[3], sb), tau1));
+      va = fmaxf(va, __fmul_rn(__fmul_rn((float)acc[1], ta), tau1));
+      vb = fmaxf(vb, __fmul_rn(__fmul_rn((float)acc[3], tb), tau1));
     }
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) {
@@ -393,8 +425,10 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
       if (i0 + r + 8 < hi) keys[i0 + r + 8] = score_key(vb);
     }
   }
-  if (rank == 0)
+  if (rank == 0) {
     for (int i = tid; i < lo + p.last; i += kSelThreads) keys[i < lo ? i : hi + i - lo] = kForced;
+    if (!p.scratch && tid < 3) keys_smem[n + tid] = 0u;  // (padding of pick_by_rank's reads)
+  }
   if (CL > 1) {
     if (p.scratch) __threadfence();
     cluster.sync();  // every CTA's keys are in place; only rank 0 goes on
@@ -403,14 +437,8 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
     __syncthreads();
   }
   if (!p.scratch) keys = keys_smem;
-  const int want = p.budget - p.first - p.last;
-  if (n <= 32 * kRegKeys) {
-    if (warp == 0) pick_in_registers<1>(keys, n, want, out, sm, 0, lane);
-  } else if (n <= kSelThreads * kRegKeys) {
-    pick_in_registers<kSelWarps>(keys, n, want, out, sm, warp, lane);
-  } else {
-    pick_in_memory(keys, n, p.budget, out, sm, tid, warp, lane);
-  }
+  if (n <= kRankKeys && !p.scratch) pick_by_rank(keys, n, p.budget, out, sm, warp, lane);
+  else pick_by_digits(keys, n, p.budget - p.first - p.last, out, sm, tid, warp, lane);
 }
 
 template <int D>
@@ -421,10 +449,10 @@ cudaError_t launch_select_d(const SelectParams& p, int n_units, int64_t max_n, i
   int cl = 1;
   while (cl < 8 && pairs * cl < 2 * num_sms && max_n / (2 * cl) >= 64) cl *= 2;
   if (pairs * cl > INT32_MAX) return cudaErrorInvalidValue;
-  const size_t smem = p.scratch ? 0 : (size_t)max_n * 4;
+  const size_t smem = p.scratch ? 0 : ((size_t)max_n + 3) * 4;
   if (smem > 32 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(select_blocks_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)(kSelectSmemKeys * 4));
+                                               (int)((kSelectSmemKeys + 3) * 4));
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
