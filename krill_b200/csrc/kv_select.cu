@@ -126,7 +126,6 @@ __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __r
 }
 
 constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;
-constexpr int kRankKeys = 256;             // most blocks that are picked by counting ranks
 constexpr uint32_t kForced = 0xffffffffu;  // above the key of every score
 
 // Order-preserving key of a score, at least 1 and below kForced (equal scores,
@@ -151,42 +150,64 @@ struct PickSmem {
   uint32_t bin, above, in_bin;
 };
 
-// Up to 256 keys: a key is picked when fewer than `budget` keys come before it
-// (larger, or equal with a lower index), which every thread counts for its two
-// against all keys, read four at a time; the picked ones' order by ballots.
-// keys: shared memory, padded with zeros to a multiple of four.
-__device__ __forceinline__ void pick_by_rank(const uint32_t* keys, int n, int budget, int32_t* out, PickSmem& sm,
-                                             int warp, int lane) {
-  bool on[2];
-  uint32_t votes[2];
+// Up to 32 * KPT keys by one warp, held in registers: bisection over the bits in
+// which the scored keys differ, until exactly `want` keys are above the
+// threshold (after about log2 n steps) or all bits are found; then the order by
+// ballots. No barrier; the CTA's other warps are done.
+template <int KPT>
+__device__ __forceinline__ void pick_in_warp(const uint32_t* keys, int n, int want, int32_t* out, int lane) {
+  uint32_t k[KPT], lo = kForced, hi = 0u;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = 64 * warp + 32 * j + lane;  // a warp's indices are consecutive
-    on[j] = false;
-    votes[j] = 0u;
-    if (64 * warp + 32 * j < n) {
-      const uint32_t k = i < n ? keys[i] : 0u;
-      int before = 0;
-#pragma unroll 4
-      for (int m = 0; m < n; m += 4) {
-        const uint4 o = *reinterpret_cast<const uint4*>(keys + m);
-        before += o.x > k || (o.x == k && m < i) ? 1 : 0;
-        before += o.y > k || (o.y == k && m + 1 < i) ? 1 : 0;
-        before += o.z > k || (o.z == k && m + 2 < i) ? 1 : 0;
-        before += o.w > k || (o.w == k && m + 3 < i) ? 1 : 0;
-      }
-      on[j] = i < n && before < budget;
-      votes[j] = __ballot_sync(0xffffffffu, on[j]);
+  for (int j = 0; j < KPT; ++j) {
+    const int i = 32 * j + lane;
+    k[j] = i < n ? keys[i] : 0u;
+    if (k[j] != 0u && k[j] != kForced) {
+      lo = min(lo, k[j]);
+      hi = max(hi, k[j]);
     }
   }
-  if (lane == 0) sm.gt[warp] = __popc(votes[0]) + __popc(votes[1]);
-  __syncthreads();
-  int at = 0;
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  uint32_t c = 0u, forced = 0u;
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) at += w < warp ? (int)sm.gt[w] : 0;
+  for (int j = 0; j < KPT; ++j) forced += k[j] == kForced ? 1u : 0u;
+  forced = __reduce_add_sync(0xffffffffu, forced);
+  const uint32_t target = (uint32_t)want + forced;  // keys to pick, forced ones among them
+  uint32_t K = kForced - 1u;  // picked: keys > K, and of those equal to K the first `need`
+  int need = 0;
+  if (want > 0) {
+    const int top = 32 - __clz(lo ^ hi);
+    K = top >= 32 ? 0u : lo >> top << top;
+    bool exact = false;
+    for (int bit = top - 1; bit >= 0 && !exact; --bit) {
+      const uint32_t cand = K | (1u << bit);
+      c = 0u;
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) c += k[j] >= cand ? 1u : 0u;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c >= target) K = cand;
+      exact = c == target;
+    }
+    if (exact) {
+      K -= 1u;
+    } else {
+      c = 0u;
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) c += k[j] > K ? 1u : 0u;
+      need = (int)(target - __reduce_add_sync(0xffffffffu, c));
+    }
+  }
   const uint32_t below = (1u << lane) - 1u;
-  if (on[0]) out[at + __popc(votes[0] & below)] = 64 * warp + lane;
-  if (on[1]) out[at + __popc(votes[0]) + __popc(votes[1] & below)] = 64 * warp + 32 + lane;
+  int gb = 0, eb = 0;
+#pragma unroll
+  for (int j = 0; j < KPT; ++j) {
+    const bool gt = k[j] > K, eq = k[j] == K && k[j] != 0u;
+    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+    const int g = gb + __popc(mg & below), e = eb + __popc(me & below);
+    if (gt || (eq && e < need)) out[g + min(e, need)] = 32 * j + lane;
+    gb += __popc(mg);
+    eb += __popc(me);
+  }
 }
 
 // Any number of keys: the threshold is found eight bits at a time, from the
@@ -196,6 +217,7 @@ __device__ __forceinline__ void pick_by_rank(const uint32_t* keys, int n, int bu
 __device__ __forceinline__ void pick_by_digits(const uint32_t* keys, int n, int want, int32_t* out, PickSmem& sm,
                                                int tid, int warp, int lane) {
   uint32_t lo = kForced, hi = 0u;
+#pragma unroll 4
   for (int i = tid; i < n; i += kSelThreads) {
     const uint32_t k = keys[i];
     if (k != kForced) {
@@ -227,6 +249,7 @@ __device__ __forceinline__ void pick_by_digits(const uint32_t* keys, int n, int 
       const int width = min(8, rem), shift = rem - width;
       for (int i = tid; i < 256; i += kSelThreads) sm.bins[i] = 0u;
       __syncthreads();
+#pragma unroll 4
       for (int i = tid; i < n; i += kSelThreads) {
         const uint32_t k = keys[i];
         if (k != kForced && (rem >= 32 || k >> rem == P >> rem)) atomicAdd(&sm.bins[(k >> shift) & 255u], 1u);
@@ -270,6 +293,7 @@ __device__ __forceinline__ void pick_by_digits(const uint32_t* keys, int n, int 
   // order: each warp a contiguous quarter
   const int per = (n + kSelThreads - 1) / kSelThreads * 32, i0 = warp * per, i1 = min(n, i0 + per);
   uint32_t ng = 0u, ne = 0u;
+#pragma unroll 4
   for (int i = i0; i < i1; i += 32) {
     const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
     ng += __popc(__ballot_sync(0xffffffffu, k > K));
@@ -288,6 +312,7 @@ __device__ __forceinline__ void pick_by_digits(const uint32_t* keys, int n, int 
       eb += sm.eq[w];
     }
   const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 4
   for (int i = i0; i < i1; i += 32) {
     const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
     const bool gt = k > K, eq = k == K && k != 0u;
@@ -425,10 +450,8 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
       if (i0 + r + 8 < hi) keys[i0 + r + 8] = score_key(vb);
     }
   }
-  if (rank == 0) {
+  if (rank == 0)
     for (int i = tid; i < lo + p.last; i += kSelThreads) keys[i < lo ? i : hi + i - lo] = kForced;
-    if (!p.scratch && tid < 3) keys_smem[n + tid] = 0u;  // (padding of pick_by_rank's reads)
-  }
   if (CL > 1) {
     if (p.scratch) __threadfence();
     cluster.sync();  // every CTA's keys are in place; only rank 0 goes on
@@ -437,8 +460,11 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
     __syncthreads();
   }
   if (!p.scratch) keys = keys_smem;
-  if (n <= kRankKeys && !p.scratch) pick_by_rank(keys, n, p.budget, out, sm, warp, lane);
-  else pick_by_digits(keys, n, p.budget - p.first - p.last, out, sm, tid, warp, lane);
+  const int want = p.budget - p.first - p.last;
+  if (n > 256) pick_by_digits(keys, n, want, out, sm, tid, warp, lane);
+  else if (warp > 0) return;
+  else if (n > 128) pick_in_warp<8>(keys, n, want, out, lane);
+  else pick_in_warp<4>(keys, n, want, out, lane);
 }
 
 template <int D>
@@ -449,10 +475,10 @@ cudaError_t launch_select_d(const SelectParams& p, int n_units, int64_t max_n, i
   int cl = 1;
   while (cl < 8 && pairs * cl < 2 * num_sms && max_n / (2 * cl) >= 64) cl *= 2;
   if (pairs * cl > INT32_MAX) return cudaErrorInvalidValue;
-  const size_t smem = p.scratch ? 0 : ((size_t)max_n + 3) * 4;
+  const size_t smem = p.scratch ? 0 : (size_t)max_n * 4;
   if (smem > 32 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(select_blocks_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)((kSelectSmemKeys + 3) * 4));
+                                               (int)(kSelectSmemKeys * 4));
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
