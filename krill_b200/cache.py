@@ -31,6 +31,9 @@ if torch is not None:
                  torch.uint8: L.DTYPE_U8}
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) if torch is not None else None
+
+
 def _dt(t) -> int:
     return _TORCH_DT[t.dtype]
 
@@ -46,7 +49,9 @@ def _ptr(t) -> Optional[int]:
 def _stream(stream) -> Optional[int]:
     if stream is not None:
         return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-    if torch is not None and torch.cuda.is_available() and torch.cuda.is_initialized():
+    if torch is not None and torch.cuda.is_initialized():
+        if _raw_stream is not None:  # the current stream's handle without a Stream object (4 us a call)
+            return _raw_stream(torch.cuda.current_device())
         return torch.cuda.current_stream().cuda_stream
     return None
 

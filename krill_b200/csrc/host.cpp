@@ -321,7 +321,13 @@ krill_status_t stage_acquire(krill_pool_t p, size_t bytes, StageSlot** out) {
   return KRILL_OK;
 }
 
-krill_status_t stage_upload(StageSlot* s, size_t bytes, cudaStream_t stream) {
+// Packets of 1 to 8 KB travel as a kernel's parameters (launch_upload says why).
+krill_status_t stage_upload(krill_pool_t p, StageSlot* s, size_t bytes, cudaStream_t stream) {
+  if (bytes > kUploadCopyBytes && bytes <= kUploadParamBytes) {
+    CUDA_TRY(launch_upload(s->h, s->d, bytes, stream));
+    p->kernels += 1;
+    return KRILL_OK;
+  }
   CUDA_TRY(cudaMemcpyAsync(s->d, s->h, bytes, cudaMemcpyHostToDevice, stream));
   return KRILL_OK;
 }
@@ -400,7 +406,7 @@ krill_status_t run_summaries(krill_pool_t p, const std::vector<SumItem>& sums, c
   const size_t bytes = sums.size() * sizeof(SumItem);
   TRY(stage_acquire(p, bytes, &slot));
   std::memcpy(slot->h, sums.data(), bytes);
-  TRY(stage_upload(slot, bytes, stream));
+  TRY(stage_upload(p, slot, bytes, stream));
   CUDA_TRY(timed_launch(p, 1, stream, [&] {
     return launch_summaries(p->geom, p->d_pool, reinterpret_cast<const SumItem*>(slot->d), (int64_t)sums.size(),
                             stream);
@@ -522,7 +528,7 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
   } else if (!p->host_only) {
     const size_t dst_bytes = n_dst * sizeof(AppendDst), sum_at = align16(dst_bytes);
     if (!sums.empty()) std::memcpy(slot->h + sum_at, sums.data(), sums.size() * sizeof(SumItem));
-    TRY(stage_upload(slot, sums.empty() ? dst_bytes : sum_at + sums.size() * sizeof(SumItem), stream));
+    TRY(stage_upload(p, slot, sums.empty() ? dst_bytes : sum_at + sums.size() * sizeof(SumItem), stream));
     CUDA_TRY(timed_launch(p, 1, stream, [&] {
       const cudaError_t e =
           launch_append(p->geom, p->d_pool, reinterpret_cast<const AppendDst*>(slot->d), lb, lc, n_seqs, n_new, k, v,
@@ -569,7 +575,7 @@ krill_status_t flush_deferred_append(krill_pool_t p, DeferredAppend& da, cudaStr
   const size_t bytes = da.dst.size() * sizeof(AppendDst);
   TRY(stage_acquire(p, bytes, &slot));
   std::memcpy(slot->h, da.dst.data(), bytes);
-  TRY(stage_upload(slot, bytes, stream));
+  TRY(stage_upload(p, slot, bytes, stream));
   TRY(launch_deferred_append(p, da, reinterpret_cast<const AppendDst*>(slot->d), stream));
   return stage_release(slot, stream);
 }
@@ -880,6 +886,34 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
     const int64_t quarter = std::max<int64_t>(1, total_sb * g.Hkv / p->num_sms / 4);
     C = 8;
     while (C < 128 && (int64_t)(2 * C) * HG <= quarter) C *= 2;
+    if (g.fmt == kFmtInt4) {
+      // The longest of the CTAs' shares sets the time: of the pieces from 8
+      // sub-blocks to twice that length take those whose rounds (pieces to a
+      // CTA, rounded up) of mean length, each with half a sub-block a warp for
+      // its start and end, come out least. 24 runs of 512 sub-blocks over 148
+      // CTAs: pieces of 16 make shares up to 1.16 times the mean, of 29 1.02;
+      // decode at that size went from 122 to 107 us, 4 queries over 16 ragged
+      // sequences from 138 to 121.
+      const int step = qt2 ? 2 : 1;
+      // layers of equal lengths are counted once
+      const int64_t per_layer = n_units / lc;
+      int64_t n_cnt = n_units;
+      if (std::equal(pl.nsb.begin() + per_layer, pl.nsb.begin() + n_units, pl.nsb.begin())) n_cnt = per_layer;
+      const double extra = 0.5 * attn_warps(g.D) / HG;
+      double best = 1e300;
+      int best_c = C;
+      for (int c = 8; c <= 2 * C; ++c) {
+        int64_t n = 0;
+        for (int64_t ui = 0; ui < n_cnt; ui += step) n += (uint32_t)(pl.nsb[ui] + c - 1) / (uint32_t)c;
+        n *= n_units / n_cnt;
+        const double cost = (double)((n + p->num_sms - 1) / p->num_sms) * ((double)total_sb / std::max<int64_t>(1, n) + extra);
+        if (cost < best) {
+          best = cost;
+          best_c = c;
+        }
+      }
+      C = best_c;
+    }
   }
   // ---- cascade items: (layer, row block, kv head) pairs cut into fragments.
   // A pair is either a shared-prefix group (rows = member sequences x GQA
@@ -1197,7 +1231,7 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
   if (p->host_only) return KRILL_OK;  // dry run: planned, nothing launched
   const bool uses_scratch = split_count > 0 || sel;
   if (uses_scratch) TRY(scratch_acquire(p, stream));
-  TRY(stage_upload(slot, total, stream));
+  TRY(stage_upload(p, slot, total, stream));
   AttnParams ap{};
   ap.pool = p->d_pool;
   ap.page_bytes = g.page_bytes;
@@ -1318,7 +1352,7 @@ krill_status_t do_select(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
     for (int64_t j = 0; j < bt_stride; ++j) bt[si * bt_stride + j] = j < (int64_t)blocks.size() ? blocks[j] : -1;
   }
   if (sp.scratch) TRY(scratch_acquire(p, stream));
-  TRY(stage_upload(slot, units_bytes + bt_bytes, stream));
+  TRY(stage_upload(p, slot, units_bytes + bt_bytes, stream));
   sp.units = reinterpret_cast<const AttnUnit*>(slot->d);
   sp.bt = reinterpret_cast<const int32_t*>(slot->d + units_bytes);
   sp.bt_stride = (int)bt_stride;
@@ -1350,7 +1384,7 @@ krill_status_t upload_bt(krill_pool_t p, const Seq& s, cudaStream_t stream, Stag
   TRY(stage_acquire(p, n * sizeof(int32_t), &slot));
   int32_t* bt = reinterpret_cast<int32_t*>(slot->h);
   for (size_t i = 0; i < n; ++i) bt[i] = i < s.blocks.size() ? s.blocks[i] : -1;
-  TRY(stage_upload(slot, n * sizeof(int32_t), stream));
+  TRY(stage_upload(p, slot, n * sizeof(int32_t), stream));
   *out = slot;
   return KRILL_OK;
 }
@@ -1893,7 +1927,7 @@ krill_status_t krill_read_rows(krill_pool_t p, int32_t n_seqs, const krill_seq_t
     const auto& blocks = pl.sv[i]->blocks;
     for (int64_t j = 0; j < bt_stride; ++j) bt[i * bt_stride + j] = j < (int64_t)blocks.size() ? blocks[j] : -1;
   }
-  TRY(stage_upload(slot, st_bytes + bt_bytes, (cudaStream_t)stream));
+  TRY(stage_upload(p, slot, st_bytes + bt_bytes, (cudaStream_t)stream));
   CUDA_TRY(launch_read_rows(p->geom, p->d_pool, reinterpret_cast<const int32_t*>(slot->d + st_bytes), (int)bt_stride,
                             reinterpret_cast<const int64_t*>(slot->d), layer_begin, layer_count, n_seqs, n_rows, keys,
                             values, dtype, (cudaStream_t)stream));

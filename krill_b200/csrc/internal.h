@@ -178,6 +178,15 @@ struct RopeTable {
 inline bool append_uses_tiles(int n_new) { return n_new >= 16; }
 inline int append_tile_chunks(int n_new, int subt) { return (n_new + subt - 1) / subt + 1; }
 
+// A small host packet written to device memory (16-byte aligned, room for a
+// multiple of 16 bytes on both sides) by a kernel that carries it as its
+// parameters: h is read before the call returns. For kUploadCopyBytes < bytes
+// <= kUploadParamBytes; a smaller packet goes as fast through a copy, which
+// the driver puts into the command stream, a larger one costs the launch more
+// than the copy engine's turn.
+constexpr size_t kUploadCopyBytes = 1024, kUploadParamBytes = 8192;
+cudaError_t launch_upload(const void* h, void* d, size_t bytes, cudaStream_t stream);
+
 // Kernels that store scales raise *large_scale when one has |s| >= 64 (the
 // one-fma dequantization is exact only below that).
 cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin,

@@ -1076,14 +1076,15 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_combine_kernel(AttnPa
   const int hq = (int)(w % p.max_cols), h = (int)(w / p.max_cols % Hkv);
   const int64_t ui = w / p.max_cols / Hkv;
   if (ui >= p.n_split_units) return;
-  const AttnUnit un = p.units[p.split_units[ui]];
+  const AttnUnit un = p.units[p.split_units[ui]];  // (written before the attention kernel began)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (hq < unit_cols(un, p.g)) combine_row<D>(p, un, h, hq, lane);
 }
 template <int D>
 cudaError_t run_combine(const AttnParams& p, cudaStream_t stream) {
   const int64_t warps = (int64_t)p.n_split_units * p.Hkv * p.max_cols;
-  attn_combine_kernel<D><<<(unsigned)((warps + kCombineWarps - 1) / kCombineWarps), 32 * kCombineWarps, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(attn_combine_kernel<D>, dim3((unsigned)((warps + kCombineWarps - 1) / kCombineWarps)),
+                          32 * kCombineWarps, stream, p);
 }
 
 // Work split inside a CTA: an item covers hg kv heads; HPR = NCW / R of them
@@ -1582,6 +1583,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) attn_tc_kernel(AttnParams p
   volatile uint32_t* tags = reinterpret_cast<volatile uint32_t*>(smem + SM::TAG_OFF);
   volatile uint32_t* stall_word = reinterpret_cast<volatile uint32_t*>(smem + SM::MISC_OFF + 8);
 
+  asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel, which waits for this grid
   const int tid = threadIdx.x;
   const int warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {

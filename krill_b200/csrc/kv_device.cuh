@@ -7,6 +7,24 @@
 namespace krill {
 namespace {
 
+// Launch of a combine kernel as the programmatic dependent of the kernel
+// before it on the stream: its blocks are there when that grid ends (it calls
+// griddepcontrol.launch_dependents at its start), and wait for the end before
+// they read what it wrote.
+template <typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, unsigned threads, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }

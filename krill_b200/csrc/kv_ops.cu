@@ -641,6 +641,22 @@ __global__ void scatter_kernel(uint8_t* __restrict__ pool, Geom geom, int layer,
   }
 }
 
+struct UploadPacket {
+  uint4 w[kUploadParamBytes / 16];
+};
+
+// A call's metadata packet, carried as the kernel's parameters. A copy of more
+// than 1 KB runs on a copy engine, whose hand-over to the next kernel is what
+// it costs: packet + a kernel reading it, back to back, take 10.4 us at 4 KB
+// by copy and 7.2 us this way (8 KB 10.6 and 7.2, 16 KB 10.7 and 9.2; 1 KB,
+// where the driver puts the bytes into the command stream, 6.2 and 6.2 to
+// 7.9). On the host the launch costs 1.2 us more than the copy at 4 KB, 2.7 us
+// at 16 KB, so the limit is 8 KB.
+__global__ void __launch_bounds__(256) upload_kernel(const __grid_constant__ UploadPacket p,
+                                                     uint4* __restrict__ d, int n) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) d[i] = p.w[i];
+}
+
 }  // namespace
 
 cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin,
@@ -737,6 +753,13 @@ cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, 
   KRILL_APPEND(8, 32)   // D=256, G=256
 #undef KRILL_APPEND
   return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_upload(const void* h, void* d, size_t bytes, cudaStream_t stream) {
+  const int n = (int)((bytes + 15) / 16);
+  upload_kernel<<<1, n < 256 ? (n + 31) / 32 * 32 : 256, 0, stream>>>(*static_cast<const UploadPacket*>(h),
+                                                                     static_cast<uint4*>(d), n);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_gather(const Geom& g, const uint8_t* pool, int layer, const int32_t* d_bt,

@@ -393,37 +393,49 @@ __device__ __forceinline__ void store_out32(void* out, int dtype, int64_t at, co
 }
 
 // Merges the fragments of split row blocks of direct causal items: one warp
-// per query row, lanes over D, records in fragment order.
+// per query row, lanes over D, records in fragment order. A row is a chain of
+// a few dependent reads, so what a read does not depend on is not before it:
+// the output row's place and the first two fragments (nearly every block has
+// two) are fetched with the maxima.
 template <int D>
 __global__ void __launch_bounds__(256) row_combine_kernel(AttnParams p) {
   constexpr int V = D / 32;
+  using Vec = typename std::conditional<V == 4, float4, float2>::type;
   const int lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const ShItem item = p.sh_items[p.sh_split[blockIdx.y]];
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= item.n_rows) return;
   const float* rec = p.partials + (int64_t)(item.rec + row) * row_rec_floats(D);
   const int64_t stride = (int64_t)item.n_rows * row_rec_floats(D);
+  const int n = item.n_frag;
+  const int32_t member = p.sh_members[item.mem_off + row / p.g];
+  auto vec = [&](int i) { return *reinterpret_cast<const Vec*>(rec + i * stride + lane * V); };
+  Vec x0 = vec(0), x1 = vec(n > 1 ? 1 : 0);
   float M = -INFINITY;
-  for (int i = 0; i < item.n_frag; ++i) M = fmaxf(M, rec[i * stride + D]);
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, rec[i * stride + D]);
+  const int64_t orow = ((int64_t)p.units[member].qo_row * p.Hq + (int64_t)item.h * p.g + row % p.g) * D;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   float Ls = 0.f, Os[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) Os[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < item.n_frag; ++i) {
+  for (int i = 0; i < n; ++i) {
     const float mi = rec[i * stride + D], li = rec[i * stride + D + 1];
+    const Vec x = x0;
+    x0 = x1;
+    if (i + 2 < n) x1 = vec(i + 2);
     const float w = mi == -INFINITY ? 0.f : exp2f(mi - M);
     Ls += (mi == -INFINITY) ? 0.f : li * w;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float oi = rec[i * stride + lane + 32 * e];
+      const float oi = reinterpret_cast<const float*>(&x)[e];
       Os[e] = (mi != -INFINITY) ? Os[e] + oi * w : Os[e];
     }
   }
   const float inv = 1.f / Ls;
-  const AttnUnit* un = p.units + p.sh_members[item.mem_off + row / p.g];
-  const int64_t orow = ((int64_t)un->qo_row * p.Hq + (int64_t)item.h * p.g + row % p.g) * D;
 #pragma unroll
-  for (int e = 0; e < V; ++e) store_out(p.out, p.out_dtype, orow + lane + 32 * e, Os[e] * inv);
+  for (int e = 0; e < V; ++e) store_out(p.out, p.out_dtype, orow + lane * V + e, Os[e] * inv);
 }
 
 template <int D, int NG, int FMT>
@@ -441,6 +453,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
     if (threadIdx.x == 0) atomicOr(p.err, kErrBadArg);
     return;
   }
+  asm volatile("griddepcontrol.launch_dependents;");  // the row combine, which waits for this grid
   auto bar = [&](int i) { return sbase + SM::BAR_OFF + 8u * (uint32_t)i; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::MISC_OFF);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(smem + SM::MISC_OFF + 4);
@@ -1538,9 +1551,8 @@ int shared_pair_capacity(const Geom& g) {
 cudaError_t launch_row_combine(const Geom& g, const AttnParams& p, cudaStream_t stream) {
   if (p.n_sh_split == 0) return cudaSuccess;
   const dim3 grid(256 / 8, (unsigned)p.n_sh_split);
-  if (g.D == 64) row_combine_kernel<64><<<grid, 256, 0, stream>>>(p);
-  else row_combine_kernel<128><<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (g.D == 64) return launch_dependent(row_combine_kernel<64>, grid, 256, stream, p);
+  return launch_dependent(row_combine_kernel<128>, grid, 256, stream, p);
 }
 
 cudaError_t launch_shared_umma(const Geom& g, const AttnParams& p, cudaStream_t stream) {

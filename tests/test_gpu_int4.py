@@ -429,3 +429,19 @@ def test_decode_step_host():
             kk, vv = (torch.cat([kv[i][j][layer], new[j]], 1) for j in range(2))
             check(out[layer, i].cuda(), ref.attend(q[layer, i][None], kk, vv, 0.125)[0], vv, pool)
     pool.close()
+
+
+@pytest.mark.parametrize("n_seqs", [128, 129, 1024, 1025])
+def test_metadata_packets_of_every_route(n_seqs):
+    """Appends and reads whose metadata packet is the largest or the first past
+    each route's limit (1 KB and 8 KB; an append destination has 8 bytes)."""
+    D = 64
+    pool = pool4(1, 1, 1, D, 64, blocks=n_seqs + 1)
+    seqs = [pool.create_sequence() for _ in range(n_seqs)]
+    g = gen(n_seqs)
+    k, v = (rows(g, (1, n_seqs, 1, 1, D), torch.float16) for _ in range(2))
+    kb.append_quantize(pool, seqs, 0, k, v)
+    got_k, got_v = kb.read_rows(pool, seqs, 0, 1, 1)
+    assert torch.equal(got_k, ref.value4(*ref.quantize4(k, 64)).half())
+    assert torch.equal(got_v, ref.value4(*ref.quantize4(v, 64)).half())
+    pool.close()
