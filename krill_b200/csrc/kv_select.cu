@@ -26,7 +26,7 @@ constexpr int kSumThreads = 128;
 template <int FMT>
 __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __restrict__ pool, Geom geom,
                                                                     const SumItem* __restrict__ items) {
-  __shared__ float mn_s[8][256], mx_s[8][256], red[4];
+  __shared__ __align__(8) float mn_s[8][256], mx_s[8][256], red[4];
   const int D = geom.D, NG = geom.NG;
   const SumItem it = items[blockIdx.x / geom.Hkv];
   const int h = blockIdx.x % geom.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -44,22 +44,31 @@ __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __r
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
       const float2 s = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(sb + q4_meta(D, NG, 0, gi, 0) + (8 * r + 2 * u) * 2)));
       const float2 z = __half22float2(u2h(*reinterpret_cast<const uint32_t*>(sb + q4_meta(D, NG, 1, gi, 0) + (8 * r + 2 * u) * 2)));
+      float lo[16], hi[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int k = e >> 2, sh = (e & 1) * 16 + ((e >> 1) & 1) * 4;  // d = 4k + h + 2 * high nibble
         const float a = fmaf((float)((w[k] >> sh) & 15u), s.x, z.x);
         const float b = fmaf((float)((w[k] >> (sh + 8)) & 15u), s.y, z.y);
-        float lo = fminf(a, b), hi = fmaxf(a, b);
+        lo[e] = fminf(a, b);
+        hi[e] = fmaxf(a, b);
+      }
+      // over the eight rows: at each step a lane keeps half of its channels and
+      // hands the other half over, so that it ends with channels 2r, 2r + 1
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-        }
-        if (r == 0) {
-          mn_s[u][64 * hh + 16 * tig + e] = lo;
-          mx_s[u][64 * hh + 16 * tig + e] = hi;
+      for (int n = 8; n >= 2; n /= 2) {
+        const bool up = (r & (n / 2)) != 0;
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+          const float l = __shfl_xor_sync(0xffffffffu, up ? lo[e] : lo[e + n], 2 * n);
+          const float m = __shfl_xor_sync(0xffffffffu, up ? hi[e] : hi[e + n], 2 * n);
+          lo[e] = fminf(up ? lo[e + n] : lo[e], l);
+          hi[e] = fmaxf(up ? hi[e + n] : hi[e], m);
         }
       }
+      const int d = 64 * hh + 16 * tig + 2 * r;
+      *reinterpret_cast<float2*>(&mn_s[u][d]) = make_float2(lo[0], lo[1]);
+      *reinterpret_cast<float2*>(&mx_s[u][d]) = make_float2(hi[0], hi[1]);
     }
   } else {
     // D/4 threads cover a token's channels, four each
