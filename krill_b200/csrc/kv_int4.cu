@@ -167,7 +167,8 @@ __device__ __forceinline__ void rope16(uint32_t (&w)[8], int c, int64_t pos, con
 
 // Appends of a few tokens (decode steps): one lane per 16 elements of a row,
 // D/16 lanes a row, K and V rows of a token side by side. Each lane's 8 code
-// bytes go straight to the pool (a byte belongs to one token).
+// bytes go straight to the pool (a byte belongs to one token). Launch latency
+// bounds it: 4.1 us for one token of 4 sequences, 16 layers, 8 heads of 64.
 template <int D, int G, int DT>
 __global__ void __launch_bounds__(256) append4_kernel(uint8_t* __restrict__ pool, Geom geom,
                                                       const AppendDst* __restrict__ dst, int layer_begin,
@@ -257,7 +258,9 @@ __device__ __forceinline__ bool tile_quantize(uint32_t (&w)[PER][8], int64_t cs,
 // touched sub-block). A sub-block that the call covers whole is built in shared
 // memory and leaves with 16-byte stores; one that it covers in part gets byte
 // stores (on a windowed pool the call's first and last chunk can be parts of
-// one sub-block, so neither may write the other's bytes).
+// one sub-block, so neither may write the other's bytes). Bound by issue, most
+// of it the quotients (about 5 instructions a code): 49 us for 2 x 2039 tokens,
+// 8 layers, 8 heads of 128, whose 171 MB take 26 us at copy bandwidth.
 template <int D, int G, int DT>
 __global__ void __launch_bounds__(256) append4_tile_kernel(uint8_t* __restrict__ pool, Geom geom,
                                                            const AppendDst* __restrict__ dst, int layer_begin,
@@ -370,6 +373,8 @@ __device__ __forceinline__ bool read_at(const uint8_t* pool, const Geom& geom, c
 // 16 elements: of K two 16-byte words, of V eight 4-byte words of the image in
 // shared memory, whose V codes are spread by 16 bytes per 512 against bank
 // conflicts. Its eight (K) lanes along D write 256 consecutive bytes a row.
+// 41 us for the rows of the append above (the same bytes, 26 us), 4.9 us for
+// the one-token one.
 template <int D, int G>
 __global__ void __launch_bounds__(256) read_rows4_kernel(const uint8_t* __restrict__ pool, Geom geom,
                                                          const int32_t* __restrict__ bt, int bt_stride,

@@ -23,6 +23,9 @@ constexpr int kSumThreads = 128;
 
 // One CTA per (sub-block, kv head). min / max of the sub-block's K values per
 // channel, partial over the threads' token subsets, joined in shared memory.
+// Runs once for a sub-block, when it fills up: 19 us for 512 x 8 of 4 bits at
+// head_dim 128, 30 us of 8 bits (20 and 37 MB: 3 and 6 us), beside 47 and 69 us
+// for their append; bound by the latency of its steps.
 template <int FMT>
 __global__ void __launch_bounds__(kSumThreads) block_summary_kernel(uint8_t* __restrict__ pool, Geom geom,
                                                                     const SumItem* __restrict__ items) {
@@ -341,7 +344,9 @@ __device__ __forceinline__ void pick_by_digits(const uint32_t* keys, int n, int 
 // to scratch, for sequences of more blocks than fit), which picks. Latency
 // bounds it: the summaries of a warp's next 16 blocks are fetched while it
 // works on the ones before (the first while the query is rounded), their block
-// ids a step earlier.
+// ids a step earlier. At head_dim 128: 11.2 us for 8 layers of 32 sequences of
+// 512 to 8192 tokens, 8 heads (28 MB, 4.3 us), 13.3 us for 4 layers of 2 of
+// 131072 tokens, 4 heads (17 MB, 2.6 us).
 template <int D>
 __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams p) {
   asm volatile("griddepcontrol.launch_dependents;");

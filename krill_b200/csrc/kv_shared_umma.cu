@@ -24,8 +24,16 @@
 //     rare O rescale is a tcgen05.ld / st round trip after the previous P·V
 //     has completed. At the end of an item they read O and write the fp32
 //     partial records.
+// Causal items (verify, chunked prefill) write the rows they finish straight to
+// the output; only row blocks cut between two CTAs leave records.
+// 512 queries of 8 sequences behind 4096 tokens of a 4-bit pool, 2 layers, 32
+// heads over 8 of 128: 814 us, 0.44 of the bf16 peak. The softmax bounds it: per
+// tile of 128 x 64 scores the exponentials alone take 512 cycles for the 719 of
+// the tile's two products, and the chain S, softmax, P.V of one half of the rows
+// overlaps only the other half's.
 // Every wait is bounded (the pool's wait_timeout_us, then 20 us after the
-// first timeout) and sets the pool's error flag; the tensor memory is released on every path.
+// first timeout) and sets the pool's error flag; the tensor memory is released
+// on every path.
 #include <atomic>
 
 #include "kv_device.cuh"
