@@ -525,6 +525,14 @@ krill_status_t do_append(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs
     deferred->k = k;
     deferred->v = v;
     deferred->pending = true;
+  } else if (p->geom.fmt == kFmtInt4 && !p->host_only && !tiled && sums.empty() &&
+             n_dst * sizeof(AppendDst) <= sizeof(InlinePacket)) {
+    // (the slot's device half is not used, its host half read before the launch returns)
+    CUDA_TRY(timed_launch(p, 1, stream, [&] {
+      return launch_append4(p->geom, p->d_pool, nullptr, slot->h, lb, lc, n_seqs, n_new, k, v, dtype, p->d_err + 1, rope,
+                            stream);
+    }));
+    p->kernels += 1;
   } else if (!p->host_only) {
     const size_t dst_bytes = n_dst * sizeof(AppendDst), sum_at = align16(dst_bytes);
     if (!sums.empty()) std::memcpy(slot->h + sum_at, sums.data(), sums.size() * sizeof(SumItem));
@@ -1927,12 +1935,12 @@ krill_status_t krill_read_rows(krill_pool_t p, int32_t n_seqs, const krill_seq_t
     const auto& blocks = pl.sv[i]->blocks;
     for (int64_t j = 0; j < bt_stride; ++j) bt[i * bt_stride + j] = j < (int64_t)blocks.size() ? blocks[j] : -1;
   }
-  TRY(stage_upload(p, slot, st_bytes + bt_bytes, (cudaStream_t)stream));
-  CUDA_TRY(launch_read_rows(p->geom, p->d_pool, reinterpret_cast<const int32_t*>(slot->d + st_bytes), (int)bt_stride,
-                            reinterpret_cast<const int64_t*>(slot->d), layer_begin, layer_count, n_seqs, n_rows, keys,
-                            values, dtype, (cudaStream_t)stream));
+  const bool inl = st_bytes + bt_bytes <= sizeof(InlinePacket);
+  if (!inl) TRY(stage_upload(p, slot, st_bytes + bt_bytes, (cudaStream_t)stream));
+  CUDA_TRY(launch_read_rows(p->geom, p->d_pool, inl ? nullptr : slot->d, slot->h, (int)bt_stride, layer_begin,
+                            layer_count, n_seqs, n_rows, keys, values, dtype, (cudaStream_t)stream));
   p->kernels += 1;
-  return stage_release(slot, (cudaStream_t)stream);
+  return inl ? KRILL_OK : stage_release(slot, (cudaStream_t)stream);
 }
 
 krill_status_t krill_prefill_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* seqs,

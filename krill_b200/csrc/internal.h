@@ -192,19 +192,29 @@ cudaError_t launch_upload(const void* h, void* d, size_t bytes, cudaStream_t str
 cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin,
                           int layer_count, int n_seqs, int n_new, const void* k, const void* v,
                           int dtype, int* large_scale, RopeTable rope, cudaStream_t stream);
-// The same for 4-bit pools (kv_int4.cu).
-cudaError_t launch_append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin, int layer_count,
-                           int n_seqs, int n_new, const void* k, const void* v, int dtype, int* large_scale,
-                           RopeTable rope, cudaStream_t stream);
+// Metadata of a small call, carried by the kernel that reads it: no copy comes
+// before the kernel (a copy of up to 1 KB and a kernel behind it take 6.2 us
+// back to back, a kernel alone 2.7). Larger ones are uploaded.
+struct InlinePacket {
+  uint32_t w[kUploadCopyBytes / 4];
+};
+// The same for 4-bit pools (kv_int4.cu). d_dst == nullptr (appends of fewer
+// than 16 tokens): the destinations are at h, in a buffer of at least
+// sizeof(InlinePacket) bytes, and travel with the kernel.
+cudaError_t launch_append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, const void* h, int layer_begin,
+                           int layer_count, int n_seqs, int n_new, const void* k, const void* v, int dtype,
+                           int* large_scale, RopeTable rope, cudaStream_t stream);
 cudaError_t launch_gather4(const Geom& g, const uint8_t* pool, int layer, const int32_t* d_bt, int64_t p0,
                            int64_t S, const GatherOut& out, cudaStream_t stream);
 cudaError_t launch_scatter4(const Geom& g, uint8_t* pool, int layer, const int32_t* d_bt, int64_t p0, int64_t S,
                             const ScatterIn& in, int* large_scale, cudaStream_t stream);
 // Dequantized rows [starts[si], + n) of (layers x sequences) of an int8 or
-// 4-bit pool, laid out like an append's input (kv_int4.cu).
-cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const int32_t* d_bt, int bt_stride,
-                             const int64_t* d_starts, int layer_begin, int layer_count, int n_seqs, int64_t n,
-                             void* keys, void* values, int dtype, cudaStream_t stream);
+// 4-bit pool, laid out like an append's input (kv_int4.cu). meta: the starts
+// (int64), padded to 16 bytes, then the block tables; nullptr: they are at h, as
+// in launch_append4.
+cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const void* meta, const void* h, int bt_stride,
+                             int layer_begin, int layer_count, int n_seqs, int64_t n, void* keys, void* values,
+                             int dtype, cudaStream_t stream);
 
 // One sub-block whose summary is to be computed, for every kv head.
 struct SumItem {

@@ -171,7 +171,8 @@ __device__ __forceinline__ void rope16(uint32_t (&w)[8], int c, int64_t pos, con
 // bounds it: 4.1 us for one token of 4 sequences, 16 layers, 8 heads of 64.
 template <int D, int G, int DT>
 __global__ void __launch_bounds__(256) append4_kernel(uint8_t* __restrict__ pool, Geom geom,
-                                                      const AppendDst* __restrict__ dst, int layer_begin,
+                                                      const AppendDst* __restrict__ dst,
+                                                      const __grid_constant__ InlinePacket inl, int layer_begin,
                                                       int layer_count, int n_seqs, int n_new,
                                                       const void* __restrict__ k, const void* __restrict__ v,
                                                       int* __restrict__ large_scale, RopeTable rope) {
@@ -191,7 +192,13 @@ __global__ void __launch_bounds__(256) append4_kernel(uint8_t* __restrict__ pool
     h = (int)(rest % geom.Hkv);
     const int64_t ls = rest / geom.Hkv;
     li = (int)(ls / n_seqs);
-    d = dst[ls * n_new + row % n_new];
+    const int64_t i = ls * n_new + row % n_new;
+    if (dst) {
+      d = dst[i];
+    } else {
+      d.block = (int32_t)inl.w[2 * i];
+      d.pos = (int32_t)inl.w[2 * i + 1];
+    }
     load16(is_k ? k : v, row * D + 16 * c, w);
   }
   if (rope.cos) rope16<D, DT>(w, c, d.pos, rope, live && is_k);
@@ -345,23 +352,25 @@ struct ReadAt {
   int64_t row0;  // output row of the sub-block's token 0
   int t_lo, t_hi;
 };
-__device__ __forceinline__ bool read_at(const uint8_t* pool, const Geom& geom, const int32_t* bt, int bt_stride,
-                                        const int64_t* starts, int layer_begin, int n_seqs, int64_t n, int n_chunks,
-                                        uint32_t b, ReadAt& at) {
+__device__ __forceinline__ bool read_at(const uint8_t* pool, const Geom& geom, const uint32_t* meta,
+                                        const InlinePacket& inl, int bt_stride, int layer_begin, int n_seqs, int64_t n,
+                                        int n_chunks, uint32_t b, ReadAt& at) {
+  auto word = [&](int64_t i) { return meta ? meta[i] : inl.w[i]; };
   const int T = geom.subt;
   const int ch = (int)(b % (uint32_t)n_chunks);
   b /= (uint32_t)n_chunks;
   const int h = (int)(b % (uint32_t)geom.Hkv);
   const int64_t ls = b / (uint32_t)geom.Hkv;
   const int si = (int)(ls % n_seqs), layer = layer_begin + (int)(ls / n_seqs);
-  const int64_t p0 = starts[si];
+  const int64_t p0 = (int64_t)((uint64_t)word(2 * si + 1) << 32 | word(2 * si));
   const int64_t cs = p0 - p0 % T + (int64_t)ch * T;
   at.t_lo = (int)max((int64_t)0, p0 - cs);
   at.t_hi = (int)min((int64_t)T, p0 + n - cs);
   if (at.t_lo >= at.t_hi) return false;
   int64_t bi = cs / kBlockTokens;
   if (geom.ring > 0) bi %= geom.ring;
-  at.sb = pool + (((int64_t)bt[(int64_t)si * bt_stride + bi] * geom.L + layer) * geom.Hkv + h) * geom.page_bytes +
+  const int32_t block = (int32_t)word((n_seqs + 1) / 2 * 4 + (int64_t)si * bt_stride + bi);
+  at.sb = pool + (((int64_t)block * geom.L + layer) * geom.Hkv + h) * geom.page_bytes +
           (cs % kBlockTokens) / T * geom.sb_bytes;
   at.row0 = (ls * geom.Hkv + h) * n + (cs - p0);
   return true;
@@ -377,14 +386,14 @@ __device__ __forceinline__ bool read_at(const uint8_t* pool, const Geom& geom, c
 // the one-token one.
 template <int D, int G>
 __global__ void __launch_bounds__(256) read_rows4_kernel(const uint8_t* __restrict__ pool, Geom geom,
-                                                         const int32_t* __restrict__ bt, int bt_stride,
-                                                         const int64_t* __restrict__ starts, int layer_begin,
-                                                         int n_seqs, int64_t n, int n_chunks, void* keys,
+                                                         const uint32_t* __restrict__ meta,
+                                                         const __grid_constant__ InlinePacket inl, int bt_stride,
+                                                         int layer_begin, int n_seqs, int64_t n, int n_chunks, void* keys,
                                                          void* values, int dtype) {
   constexpr int LPT = D / 16, NG = D / G, HALF = q4_half(D, NG), CODES = 32 * D;
   __shared__ __align__(16) uint8_t img[2 * HALF + CODES / 32];
   ReadAt at;
-  if (!read_at(pool, geom, bt, bt_stride, starts, layer_begin, n_seqs, n, n_chunks, blockIdx.x, at)) return;
+  if (!read_at(pool, geom, meta, inl, bt_stride, layer_begin, n_seqs, n, n_chunks, blockIdx.x, at)) return;
   // image: K half, V scales and zeros, V codes (spread)
   constexpr int VMETA = HALF, VCODES = HALF + 256 * NG;
   for (int i = threadIdx.x; i < 2 * HALF / 16; i += 256) {
@@ -468,14 +477,14 @@ __global__ void __launch_bounds__(256) read_rows4_kernel(const uint8_t* __restri
 
 // The same of an int8 pool.
 __global__ void __launch_bounds__(256) read_rows8_kernel(const uint8_t* __restrict__ pool, Geom geom,
-                                                         const int32_t* __restrict__ bt, int bt_stride,
-                                                         const int64_t* __restrict__ starts, int layer_begin,
-                                                         int n_seqs, int64_t n, int n_chunks, void* keys,
+                                                         const uint32_t* __restrict__ meta,
+                                                         const __grid_constant__ InlinePacket inl, int bt_stride,
+                                                         int layer_begin, int n_seqs, int64_t n, int n_chunks, void* keys,
                                                          void* values, int dtype) {
   extern __shared__ __align__(16) uint8_t img8[];
   const int D = geom.D, NG = geom.NG, LPT = D / 16;
   ReadAt at;
-  if (!read_at(pool, geom, bt, bt_stride, starts, layer_begin, n_seqs, n, n_chunks, blockIdx.x, at)) return;
+  if (!read_at(pool, geom, meta, inl, bt_stride, layer_begin, n_seqs, n, n_chunks, blockIdx.x, at)) return;
   for (int i = threadIdx.x; i < (int)(geom.sb_bytes / 16); i += 256)
     reinterpret_cast<uint4*>(img8)[i] = reinterpret_cast<const uint4*>(at.sb)[i];
   __syncthreads();
@@ -571,8 +580,8 @@ __global__ void scatter4_kernel(uint8_t* __restrict__ pool, Geom geom, int layer
 }
 
 template <int D, int G, int DT>
-cudaError_t append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin, int layer_count,
-                    int n_seqs, int n_new, const void* k, const void* v, int* large_scale, RopeTable rope,
+cudaError_t append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, const InlinePacket& inl, int layer_begin,
+                    int layer_count, int n_seqs, int n_new, const void* k, const void* v, int* large_scale, RopeTable rope,
                     cudaStream_t stream) {
   if (append_uses_tiles(n_new)) {
     const int n_chunks = append_tile_chunks(n_new, g.subt);
@@ -584,20 +593,22 @@ cudaError_t append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int la
   }
   const int64_t threads = (int64_t)layer_count * n_seqs * g.Hkv * n_new * (D / 8);
   append4_kernel<D, G, DT><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(
-      pool, g, d_dst, layer_begin, layer_count, n_seqs, n_new, k, v, large_scale, rope);
+      pool, g, d_dst, inl, layer_begin, layer_count, n_seqs, n_new, k, v, large_scale, rope);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, int layer_begin, int layer_count,
-                           int n_seqs, int n_new, const void* k, const void* v, int dtype, int* large_scale,
-                           RopeTable rope, cudaStream_t stream) {
+cudaError_t launch_append4(const Geom& g, uint8_t* pool, const AppendDst* d_dst, const void* h, int layer_begin,
+                           int layer_count, int n_seqs, int n_new, const void* k, const void* v, int dtype,
+                           int* large_scale, RopeTable rope, cudaStream_t stream) {
+  static const InlinePacket none{};
+  const InlinePacket& inl = d_dst ? none : *static_cast<const InlinePacket*>(h);
 #define KRILL_APPEND4(DD, GG)                                                                               \
   if (g.D == DD && g.G == GG)                                                                               \
-    return dtype == 0 ? append4<DD, GG, 0>(g, pool, d_dst, layer_begin, layer_count, n_seqs, n_new, k, v,   \
+    return dtype == 0 ? append4<DD, GG, 0>(g, pool, d_dst, inl, layer_begin, layer_count, n_seqs, n_new, k, v, \
                                            large_scale, rope, stream)                                       \
-                      : append4<DD, GG, 1>(g, pool, d_dst, layer_begin, layer_count, n_seqs, n_new, k, v,   \
+                      : append4<DD, GG, 1>(g, pool, d_dst, inl, layer_begin, layer_count, n_seqs, n_new, k, v, \
                                            large_scale, rope, stream);
   KRILL_APPEND4(64, 64)
   KRILL_APPEND4(128, 64)
@@ -622,15 +633,18 @@ cudaError_t launch_scatter4(const Geom& g, uint8_t* pool, int layer, const int32
   return cudaGetLastError();
 }
 
-cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const int32_t* d_bt, int bt_stride,
-                             const int64_t* d_starts, int layer_begin, int layer_count, int n_seqs, int64_t n,
-                             void* keys, void* values, int dtype, cudaStream_t stream) {
+cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const void* meta, const void* h, int bt_stride,
+                             int layer_begin, int layer_count, int n_seqs, int64_t n, void* keys, void* values,
+                             int dtype, cudaStream_t stream) {
+  static const InlinePacket none{};
+  const InlinePacket& inl = meta ? none : *static_cast<const InlinePacket*>(h);
+  const uint32_t* words = static_cast<const uint32_t*>(meta);
   const int64_t n_chunks = (n + g.subt - 1) / g.subt + 1;
   const int64_t blocks = (int64_t)layer_count * n_seqs * g.Hkv * n_chunks;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
 #define KRILL_READ4(DD, GG)                                                                                \
   if (g.fmt == kFmtInt4 && g.D == DD && g.G == GG)                                                         \
-    read_rows4_kernel<DD, GG><<<(unsigned)blocks, 256, 0, stream>>>(pool, g, d_bt, bt_stride, d_starts,    \
+    read_rows4_kernel<DD, GG><<<(unsigned)blocks, 256, 0, stream>>>(pool, g, words, inl, bt_stride,        \
                                                                     layer_begin, n_seqs, n, (int)n_chunks, \
                                                                     keys, values, dtype);
   KRILL_READ4(64, 64)
@@ -641,7 +655,7 @@ cudaError_t launch_read_rows(const Geom& g, const uint8_t* pool, const int32_t* 
 #undef KRILL_READ4
   if (g.fmt != kFmtInt4)
     read_rows8_kernel<<<(unsigned)blocks, 256, (size_t)g.sb_bytes, stream>>>(
-        pool, g, d_bt, bt_stride, d_starts, layer_begin, n_seqs, n, (int)n_chunks, keys, values, dtype);
+        pool, g, words, inl, bt_stride, layer_begin, n_seqs, n, (int)n_chunks, keys, values, dtype);
   return cudaGetLastError();
 }
 

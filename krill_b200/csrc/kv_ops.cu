@@ -665,7 +665,7 @@ cudaError_t launch_append(const Geom& g, uint8_t* pool, const AppendDst* d_dst, 
   const int64_t warps = (int64_t)layer_count * n_seqs * g.Hkv * n_new;
   if (warps == 0) return cudaSuccess;
   if (g.fmt == kFmtInt4)
-    return launch_append4(g, pool, d_dst, layer_begin, layer_count, n_seqs, n_new, k, v, dtype, large_scale, rope,
+    return launch_append4(g, pool, d_dst, nullptr, layer_begin, layer_count, n_seqs, n_new, k, v, dtype, large_scale, rope,
                           stream);
   const int threads = 256;
   const int64_t blocks = (warps * 32 + threads - 1) / threads;
