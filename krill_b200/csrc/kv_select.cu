@@ -394,6 +394,10 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
   int i0 = lo + 16 * (rank * kSelWarps + warp);
   int ba = block_of(i0 + r), bb = block_of(i0 + r + 8);
   int ba_n = block_of(i0 + step + r), bb_n = block_of(i0 + step + r + 8);
+  // The first CTA's shared memory may be written once that CTA is known to have
+  // started: every CTA arrives here and waits before its first key, with the
+  // rounding of the query between. (The return above is the whole cluster's.)
+  if (CL > 1) cluster.barrier_arrive();
   // ---- the query heads in whole numbers, one warp per head (two rounds) ----
   constexpr int QR = 8 / kSelWarps;
   float x[QR][D / 32];
@@ -431,6 +435,7 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectParams
   const bool has0 = 2 * tig < g, has1 = 2 * tig + 1 < g;
   uint32_t* keys = p.scratch ? p.scratch + (int64_t)uid * p.scratch_stride
                              : cluster.map_shared_rank(keys_smem, 0);
+  if (CL > 1) cluster.barrier_wait();
   for (; i0 < hi; i0 += step) {
     int acc[4] = {0, 0, 0, 0};
 #pragma unroll

@@ -1,0 +1,36 @@
+"""Orderings that a run cannot show reliably, checked in the kernels' source:
+what a lucky schedule hides is still in the text. CPU only."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "krill_b200", "csrc")
+
+
+def code(name):
+    """A source file without its comments."""
+    text = open(os.path.join(CSRC, name)).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def body(text, signature):
+    """The braces' content of the function that `signature` starts."""
+    at = text.index("{", text.index(signature))
+    depth = 0
+    for i in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[at:i]
+    raise AssertionError("unbalanced braces")
+
+
+def test_block_choice_waits_for_its_cluster_before_remote_stores():
+    """A CTA's shared memory may be written by the other CTAs of its cluster
+    only once it is known to have started: a cluster barrier stands between the
+    kernel's entry and the first store through map_shared_rank."""
+    text = body(code("kv_select.cu"), "select_blocks_kernel(SelectParams p)")
+    first = text.index("keys[", text.index("map_shared_rank"))
+    arrive, wait = text.find("cluster.barrier_arrive("), text.find("cluster.barrier_wait(")
+    assert 0 <= arrive < wait < first
+    # and no CTA leaves between the two, or the others would wait for it
+    assert "return" not in text[arrive:wait]
