@@ -1519,7 +1519,8 @@ __device__ __forceinline__ void produce_wide(const AttnParams& p, uint8_t* stage
   auto source = [&](const AttnItem& item, int layer, int si, int rd, int i) {
     const int h = item.h0 + rd * HPR + i % HPR;
     int sb = item.sb_begin + i / HPR;
-    if (SEL) sb = __ldg(p.sel + ((int64_t)item.unit * Hkv + h) * p.sel_stride + sb);
+    // (not through the read-only path: the choice may still write when this grid starts)
+    if (SEL) sb = __ldcg(p.sel + ((int64_t)item.unit * Hkv + h) * p.sel_stride + sb);
     int bi = sb / SPB;
     if (p.ring > 0) bi %= p.ring;
     const int b = __ldg(p.bt + (int64_t)si * p.bt_stride + bi);

@@ -1,4 +1,5 @@
-"""Block choice over clusters of every size."""
+"""Block choice over clusters of every size, and picked blocks of consecutive
+calls."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -8,8 +9,21 @@ if not torch.cuda.is_available():  # pragma: no cover
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
 import krill_b200 as kb  # noqa: E402
+from tests import _int4 as ref  # noqa: E402
 from tests.test_gpu_int4 import gen  # noqa: E402
-from tests.test_gpu_sparse import INT4, check_pick, make  # noqa: E402
+from tests.test_gpu_sparse import INT4, INT8, check_pick, check_sparse, make  # noqa: E402
+
+
+def check_step(out, q, kv, lens, scale, budget, first, last, pool):
+    """A sparse step's output against attention over the blocks that the plain
+    restatement picks for its query."""
+    L, S, H = out.shape[0], out.shape[1], pool.num_kv_heads
+    want = torch.full((L, S, H, budget), -1, dtype=torch.int32)
+    for layer in range(L):
+        for i in range(S):
+            for h, blocks in enumerate(ref.pick(q[layer, i], kv[i][0][layer], lens[i], 64, budget, first, last)):
+                want[layer, i, h, :len(blocks)] = torch.tensor(blocks, dtype=torch.int32)
+    check_sparse(out, want, q, kv, lens, 64, scale, pool)
 
 
 @pytest.mark.parametrize("layers,hkv,lens", [
@@ -29,4 +43,23 @@ def test_choice_over_clusters(layers, hkv, lens):
     got = [kb.select_blocks(pool, seqs, 0, q, 11, 1, 2) for q in qs]
     for q, picked in zip(qs, got):
         check_pick(picked, q, kv, lens, 64, 11, 1, 2)
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, INT8])
+def test_consecutive_choices_into_one_buffer(fmt):
+    """Sparse steps back to back whose choices differ and go to the same
+    scratch: each attends its own blocks, none the step's before it."""
+    g = gen(41)
+    lens, D, H = [4000, 3300, 4031], 64, 4
+    pool, seqs, kv = make(fmt, 2, H, H, D, 64, lens, torch.float16, g)
+    n = 24
+    qs = [(3 * torch.randn(2, 3, H, D, device="cuda", generator=g)).half() for _ in range(n)]
+    outs = [torch.empty(2, 3, H, D, device="cuda") for _ in range(n)]
+    torch.cuda.synchronize()
+    for q, o in zip(qs, outs):
+        kb.sparse_decode_attention(pool, seqs, 0, q, o, 0.125, 6, 1, 1)
+    torch.cuda.synchronize()
+    for q, o in zip(qs, outs):
+        check_step(o, q, kv, lens, 0.125, 6, 1, 1, pool)
     pool.close()

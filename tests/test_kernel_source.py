@@ -34,3 +34,12 @@ def test_block_choice_waits_for_its_cluster_before_remote_stores():
     assert 0 <= arrive < wait < first
     # and no CTA leaves between the two, or the others would wait for it
     assert "return" not in text[arrive:wait]
+
+
+def test_picked_blocks_are_read_coherently():
+    """The sparse decode kernel is resident while the choice before it still
+    writes the picked blocks, so they may not be read through the read-only
+    path (__ldg), whose data must not change while a kernel runs."""
+    text = code("kv_attn.cuh")
+    assert "p.sel" in text
+    assert not re.search(r"__ldg\(\s*p\.sel\b", text)
