@@ -415,8 +415,8 @@ krill_status_t krill_seq_snapshot_dequantized(krill_pool_t pool, krill_seq_t seq
  * append's layout, keys / values [layer_count][n_seqs][Hkv][n_rows][D] of
  * dtype F16, BF16 or F32 (either may be NULL; 16-byte aligned), each value
  * rounded once to it (int8 pools: the reference's two f16 roundings come
- * first). starts: host array, or NULL for the first retained row of each
- * sequence. int8 and 4-bit pools. */
+ * first). starts: host array, or NULL for the first row of each sequence that
+ * every layer of the call retains. int8 and 4-bit pools. */
 krill_status_t krill_read_rows(krill_pool_t pool, int32_t n_seqs, const krill_seq_t* seqs,
                                int32_t layer_begin, int32_t layer_count, const int64_t* starts,
                                int64_t n_rows, void* keys, void* values, int32_t dtype, void* stream);

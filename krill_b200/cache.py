@@ -431,8 +431,8 @@ def read_rows(pool: KVPool, seqs, layer_begin: int, layer_count: int, n_rows: in
               keys=None, values=None, stream=None):
     """Cached rows [starts[i], starts[i] + n_rows) of each sequence, dequantized:
     (keys, values) [layer_count, n_seqs, Hkv, n_rows, D], f16 unless ``dtype``
-    (or given outputs) say otherwise. ``starts`` defaults to the first retained
-    row (krill_read_rows)."""
+    (or given outputs) say otherwise. ``starts`` defaults to the first row that
+    every layer retains (krill_read_rows)."""
     shape = (layer_count, len(seqs), pool.num_kv_heads, max(0, n_rows), pool.head_dim)
     dtype = dtype or (keys.dtype if keys is not None else torch.float16)
     dev = torch.device("cuda", pool.device)

@@ -1913,16 +1913,22 @@ krill_status_t krill_read_rows(krill_pool_t p, int32_t n_seqs, const krill_seq_t
   Plan& pl = p->plan;
   pl.sv.resize(n_seqs);
   int64_t bt_stride = 1;
+  std::vector<int64_t> first((size_t)n_seqs);  // first row to read of each sequence
   for (int i = 0; i < n_seqs; ++i) {
     TRY(seq_get(p, seqs[i], &pl.sv[i]));
     bt_stride = std::max<int64_t>(bt_stride, (int64_t)pl.sv[i]->blocks.size());
-    for (int L = layer_begin; L < layer_begin + layer_count; ++L) {
-      int64_t p0, S;
+    int64_t p0, S;
+    first[i] = starts ? starts[i] : 0;
+    // by default the first row that every layer retains
+    for (int L = layer_begin; !starts && L < layer_begin + layer_count; ++L) {
       layer_span(p, *pl.sv[i], L, &p0, &S);
-      const int64_t start = starts ? starts[i] : p0;
-      if (start < p0 || n_rows > p0 + S - start)
+      first[i] = std::max(first[i], p0);
+    }
+    for (int L = layer_begin; L < layer_begin + layer_count; ++L) {
+      layer_span(p, *pl.sv[i], L, &p0, &S);
+      if (first[i] < p0 || n_rows > p0 + S - first[i])
         return fail(KRILL_ERR_INVALID, "rows [%lld, %lld) of sequence %d are not cached (layer %d holds [%lld, %lld))",
-                    (long long)start, (long long)(start + n_rows), i, L, (long long)p0, (long long)(p0 + S));
+                    (long long)first[i], (long long)(first[i] + n_rows), i, L, (long long)p0, (long long)(p0 + S));
     }
   }
   TRY(require_device(p));
@@ -1930,12 +1936,9 @@ krill_status_t krill_read_rows(krill_pool_t p, int32_t n_seqs, const krill_seq_t
   const size_t bt_bytes = (size_t)n_seqs * bt_stride * sizeof(int32_t);
   StageSlot* slot = nullptr;
   TRY(stage_acquire(p, st_bytes + bt_bytes, &slot));
-  int64_t* st = reinterpret_cast<int64_t*>(slot->h);
+  std::memcpy(slot->h, first.data(), (size_t)n_seqs * sizeof(int64_t));
   int32_t* bt = reinterpret_cast<int32_t*>(slot->h + st_bytes);
   for (int i = 0; i < n_seqs; ++i) {
-    int64_t p0, S;
-    layer_span(p, *pl.sv[i], layer_begin, &p0, &S);
-    st[i] = starts ? starts[i] : p0;
     const auto& blocks = pl.sv[i]->blocks;
     for (int64_t j = 0; j < bt_stride; ++j) bt[i * bt_stride + j] = j < (int64_t)blocks.size() ? blocks[j] : -1;
   }
