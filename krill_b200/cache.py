@@ -433,6 +433,8 @@ def read_rows(pool: KVPool, seqs, layer_begin: int, layer_count: int, n_rows: in
     (keys, values) [layer_count, n_seqs, Hkv, n_rows, D], f16 unless ``dtype``
     (or given outputs) say otherwise. ``starts`` defaults to the first row that
     every layer retains (krill_read_rows)."""
+    if starts is not None and len(starts) != len(seqs):
+        raise ValueError(f"starts must hold one row for each of the {len(seqs)} sequences")
     shape = (layer_count, len(seqs), pool.num_kv_heads, max(0, n_rows), pool.head_dim)
     dtype = dtype or (keys.dtype if keys is not None else torch.float16)
     dev = torch.device("cuda", pool.device)

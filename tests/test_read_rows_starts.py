@@ -44,3 +44,11 @@ def test_no_common_row():
     p, s, arr = make(kb.KV_INT4, [64, 600])
     assert L.lib.krill_read_rows(p.handle, 1, arr, 0, 2, None, 1, None, None, L.DTYPE_F16, None) == L.KRILL_ERR_INVALID
     assert "not cached" in L.last_error()
+
+
+@pytest.mark.parametrize("starts", [[5], [], [1, 2, 3]])
+def test_one_start_for_each_sequence(starts):
+    """Too few starts are refused, not filled up with zeros."""
+    p, s, _ = make(kb.KV_INT4, [128, 128])
+    with pytest.raises(ValueError, match="starts"):
+        kb.read_rows(p, [s, s], 0, 2, 1, starts=starts)
