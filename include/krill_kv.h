@@ -94,10 +94,12 @@ enum {
  *   scale = f16(f32(max - min) / 15), zero = f16(min)
  *   code  = clip(round-half-even((x - zero) / scale), 0, 15), in f32 (scale 0: 0)
  *   value = code * scale + zero in f32
- * Inputs beyond +-61440 saturate and NaN counts as 0, so a 4-bit cache never
- * holds an infinity or NaN. Every call of this header takes 4-bit pools except
- * the disk tier; snapshots hold one code (0..15) per byte. KRILL_QUANT_F32
- * and KRILL_ATTN_TENSOR_CORE only; k/v of an append must be 16-byte aligned. */
+ * Inputs beyond +-61440 saturate and NaN counts as 0, and of restored rows a
+ * zero is kept within +-61440, a scale where all sixteen values are finite in
+ * f16, NaN as 0, so a 4-bit cache never holds an infinity or NaN. Every call
+ * of this header takes 4-bit pools except the disk tier; snapshots hold one
+ * code (0..15) per byte. KRILL_QUANT_F32 and KRILL_ATTN_TENSOR_CORE only; k/v
+ * of an append must be 16-byte aligned. */
 enum { KRILL_KV_INT8 = 0, KRILL_KV_BF16 = 1, KRILL_KV_INT4 = 2 };
 
 typedef struct krill_pool_s* krill_pool_t;

@@ -7,8 +7,9 @@
 //   value = c * s + z in f32, rounded once to the type it is read in.
 // Inputs beyond +-61440 saturate and NaN counts as 0, so that no stored scale
 // or zero is infinite or NaN and every value is within f16's range
-// (15 * f16(122880 / 15) - 61440 = 61440); a masked token can then never
-// contribute more than its weight of zero.
+// (15 * f16(122880 / 15) - 61440 = 61440); restored scales and zeros are kept
+// there too (sane_meta4). A masked token can then never contribute more than
+// its weight of zero.
 // The quotient (x - z) / s is the correctly rounded one: q = t * RN(1/s) is
 // corrected by its residual, q + (t - q s) RN(1/s), one fma each (P. Markstein,
 // IBM J. Res. Dev. 34(1), 1990, theorem on division with a correctly rounded
@@ -548,6 +549,21 @@ __global__ void gather4_kernel(const uint8_t* __restrict__ pool, Geom geom, int 
   }
 }
 
+// A restored group's scale and zero, which may be any f16: the zero is kept
+// within +-61440 and the scale where all sixteen values are finite in f16, NaN
+// as 0. What an append stores passes unchanged (its values end below 61440 + 16
+// + 15 * 2, the roundings of z and s).
+__device__ __forceinline__ void sane_meta4(uint16_t& s16, uint16_t& z16) {
+  float z = __half2float(__ushort_as_half(z16));
+  if (!(fabsf(z) <= kSat4)) {
+    z = sane4(z);
+    z16 = __half_as_ushort(__float2half_rn(z));
+  }
+  const float s = __half2float(__ushort_as_half(s16));
+  const float hi = __fdiv_rz(65504.0f - z, 15.0f), lo = __fdiv_rz(-65504.0f - z, 15.0f);
+  if (!(s >= lo && s <= hi)) s16 = isnan(s) ? 0 : __half_as_ushort(__float2half_rz(s > hi ? hi : lo));
+}
+
 // Snapshot layout -> pages (restore, scatter-back); codes are taken modulo 16.
 __global__ void scatter4_kernel(uint8_t* __restrict__ pool, Geom geom, int layer, const int32_t* __restrict__ bt,
                                 int64_t p0, int64_t S, ScatterIn in, int* __restrict__ large_scale) {
@@ -571,10 +587,11 @@ __global__ void scatter4_kernel(uint8_t* __restrict__ pool, Geom geom, int layer
 #pragma unroll
   for (int j = 0; j < 8; ++j) sb[is_k ? q4_kbyte(D, t, c, j) : q4_vbyte(D, NG, t, c, j)] = chunk_byte(codes, is_k, j);
   if ((16 * c) % geom.G == 0) {
-    const uint16_t s16 = (is_k ? in.key_scales : in.value_scales)[irow * NG + gi];
+    uint16_t s16 = (is_k ? in.key_scales : in.value_scales)[irow * NG + gi];
+    uint16_t z16 = (is_k ? in.key_zeros : in.value_zeros)[irow * NG + gi];
+    sane_meta4(s16, z16);
     *reinterpret_cast<uint16_t*>(sb + q4_meta(D, NG, a, gi, t)) = s16;
-    *reinterpret_cast<uint16_t*>(sb + q4_meta(D, NG, a + 1, gi, t)) =
-        (is_k ? in.key_zeros : in.value_zeros)[irow * NG + gi];
+    *reinterpret_cast<uint16_t*>(sb + q4_meta(D, NG, a + 1, gi, t)) = z16;
     if ((s16 & 0x7fffu) >= 0x5400u) atomicOr(large_scale, 1);
   }
 }
