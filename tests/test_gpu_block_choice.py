@@ -1,5 +1,7 @@
 """Block choice over clusters of every size, and picked blocks of consecutive
-calls."""
+calls and of several streams."""
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -62,4 +64,47 @@ def test_consecutive_choices_into_one_buffer(fmt):
     torch.cuda.synchronize()
     for q, o in zip(qs, outs):
         check_step(o, q, kv, lens, 0.125, 6, 1, 1, pool)
+    pool.close()
+
+
+def test_streams_with_work_of_their_own():
+    """Sparse steps of different queries, budgets and sequences and split dense
+    decodes, interleaved over four streams: the pool's scratch (picked blocks,
+    partial records) is one buffer, laid out anew by each call."""
+    g = gen(42)
+    lens, D, H, hq = [20001, 9000, 12345], 64, 2, 8
+    pool, seqs, kv = make(INT4, 1, H, hq, D, 64, lens, torch.float16, g)
+    groups = [[0, 1, 2], [2, 0], [1], [0]]
+    budgets = [40, 7, 90, 21]
+    streams = [torch.cuda.Stream() for _ in groups]
+    steps = []  # (stream, sequences, budget or None, q, out)
+    for _ in range(6):
+        for s, who, budget in zip(streams, groups, budgets):
+            for b in (budget, None):
+                q = (2 * torch.randn(1, len(who), hq, D, device="cuda", generator=g)).half()
+                steps.append((s, who, b, q, torch.empty(1, len(who), hq, D, device="cuda")))
+    # the scratch has its final size before the streams start: growing it waits for the device
+    for s, who, b, q, o in steps[:8]:
+        if b:
+            kb.sparse_decode_attention(pool, [seqs[i] for i in who], 0, q, o, 0.125, b, 1, 2)
+        else:
+            kb.decode_attention(pool, [seqs[i] for i in who], 0, q, o, 0.125)
+    for step in steps:
+        step[4].fill_(math.nan)
+    torch.cuda.synchronize()
+    for s, who, b, q, o in steps:
+        if b:
+            kb.sparse_decode_attention(pool, [seqs[i] for i in who], 0, q, o, 0.125, b, 1, 2, stream=s)
+        else:
+            kb.decode_attention(pool, [seqs[i] for i in who], 0, q, o, 0.125, stream=s)
+    torch.cuda.synchronize()
+    for s, who, b, q, o in steps:
+        mine, n = [kv[i] for i in who], [lens[i] for i in who]
+        if b:
+            check_step(o, q, mine, n, 0.125, b, 1, 2, pool)
+            continue
+        for j in range(len(who)):
+            want = ref.attend(q[0, j][None], mine[j][0][0], mine[j][1][0], 0.125)[0]
+            err = (o[0, j].double() - want).abs()
+            assert (err <= ref.tolerance(mine[j][1][0], o.dtype, want)).all(), f"{err.max().item():.3e}"
     pool.close()
