@@ -577,8 +577,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) attn_shared_umma_kernel(AttnPar
     {
       uint32_t leader;
       asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+      // (every lane's test: what the barrier orders holds for lanes that saw it
+      // complete, and the issuing one must be among them)
       auto ready = [&](uint32_t b, uint32_t phase) {
-        return __any_sync(0xffffffffu, mbar_test_wait(b, phase) != 0);
+        return __all_sync(0xffffffffu, mbar_test_wait(b, phase) != 0);
       };
       constexpr uint32_t idS = umma_idesc(128, 64), idO = umma_idesc(128, D);
       uint32_t cnt0 = 0, cnt1 = 0;  // tiles processed by each half

@@ -43,3 +43,12 @@ def test_picked_blocks_are_read_coherently():
     text = code("kv_attn.cuh")
     assert "p.sel" in text
     assert not re.search(r"__ldg\(\s*p\.sel\b", text)
+
+
+def test_mma_issuer_goes_by_its_own_observation():
+    """What a barrier's completion orders holds for the threads that observed
+    it. The lane that issues the MMAs must be one of them: every lane's test has
+    to have succeeded, not any lane's."""
+    text = body(code("kv_shared_umma.cu"), "attn_shared_umma_kernel(AttnParams p)")
+    polled = re.findall(r"__(any|all)_sync\(\s*0xffffffffu\s*,\s*mbar_\w+", text)
+    assert polled and set(polled) == {"all"}
