@@ -108,3 +108,17 @@ def test_streams_with_work_of_their_own():
             err = (o[0, j].double() - want).abs()
             assert (err <= ref.tolerance(mine[j][1][0], o.dtype, want)).all(), f"{err.max().item():.3e}"
     pool.close()
+
+
+@pytest.mark.parametrize("blocks", [8193, 12289, 49152])
+def test_many_keys_in_shared_memory(blocks):
+    """Sequences whose keys take more than 32 KB, more than 48 KB and all of the
+    shared memory that a choice may use."""
+    n = 64 * blocks - 5
+    g = gen(blocks)
+    pool, seqs, kv = make(INT4, 1, 1, 2, 64, 64, [n], torch.float16, g, chunk=400000)
+    q = torch.randn(1, 1, 2, 64, device="cuda", generator=g).half()
+    picked = kb.select_blocks(pool, seqs, 0, q, 33, 1, 2)
+    check_pick(picked, q, kv, [n], 64, 33, 1, 2)
+    assert pool.device_error() == 0
+    pool.close()

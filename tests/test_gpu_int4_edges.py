@@ -1,5 +1,5 @@
 """4-bit pools at the edges of the format: restored metadata that no append
-would store."""
+would store, and what the prompt path's f16 values cost against the format's."""
 import math
 
 import pytest
@@ -12,7 +12,7 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 import krill_b200 as kb  # noqa: E402
 from tests import _int4 as ref  # noqa: E402
-from tests.test_gpu_int4 import check, gen, pool4, rows  # noqa: E402
+from tests.test_gpu_int4 import check, fill, gen, pool4, rows  # noqa: E402
 
 BAD = [math.inf, -math.inf, math.nan, 65504.0, -65504.0]
 
@@ -93,4 +93,93 @@ def test_masked_token_with_bad_metadata(D, G, hq, hkv, nq, bad):
             kk, vv = kk.half().double(), vv.half().double()
         want = ref.attend(q[0, 0], kk, vv, scale, seen)[:before]
         check(out[0, 0, :before], want, vv * 2, pool)
+    pool.close()
+
+
+def test_scatter_back():
+    """Stacked sequences grown by new rows and written back."""
+    D, G, hkv, steps = 128, 64, 2, 5
+    g = gen(52)
+    pool = pool4(2, hkv, 4, D, G, blocks=32)
+    lens = [70, 300, 1]
+    seqs, kv = fill(pool, lens, torch.bfloat16, g, 2)
+    for layer in range(2):
+        st = kb.stack_caches_left_padded_quantized(pool, seqs, layer)
+        s_max = st.keys.shape[2]
+        new = snapshot(g, 3 * hkv, steps, D, G, torch.bfloat16)
+        grown = kb.QuantizedKVSnapshot(*[
+            torch.cat([getattr(st, name), getattr(new, name).reshape(3, hkv, steps, -1)], 2).contiguous()
+            for name in ("keys", "values", "key_scales", "key_zeros", "value_scales", "value_zeros")])
+        kb.scatter_back(pool, seqs, layer, grown, lens, s_max, steps)
+        for i, n in enumerate(lens):
+            got = seqs[i].quantized_snapshot(layer)
+            for name in ("keys", "values", "key_scales", "key_zeros", "value_scales", "value_zeros"):
+                assert torch.equal(getattr(got, name), getattr(grown, name)[i, :, s_max - n:])
+    q = torch.randn(2, 3, 4, D, device="cuda", generator=g).to(torch.bfloat16)
+    out = torch.empty(2, 3, 4, D, device="cuda")
+    kb.decode_attention(pool, seqs, 0, q, out, 0.09)
+    for layer in range(2):
+        for i in range(3):
+            x = seqs[i].quantized_snapshot(layer)
+            k, v = ref.value4(x.keys, x.key_scales, x.key_zeros), ref.value4(x.values, x.value_scales, x.value_zeros)
+            check(out[layer, i], ref.attend(q[layer, i][None], k, v, 0.09)[0], v, pool)
+    pool.close()
+
+
+@pytest.mark.parametrize("D,G", [(64, 64), (128, 64), (128, 128), (256, 64), (256, 256)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_read_rows_int8(D, G, dtype):
+    """Rows of an int8 pool read back: the format's two f16 roundings, then one
+    to the output's type."""
+    layers, hkv, lens = 2, 2, [300, 77, 513]
+    g = gen(D + G)
+    pool = kb.KVPool(layers, hkv, 4, D, num_blocks=16, group_size=G)
+    seqs, kept = [], []
+    for n in lens:
+        seqs.append(pool.create_sequence())
+        k, v = (rows(g, (layers, 1, hkv, n, D), dtype) for _ in range(2))
+        kb.append_quantize(pool, [seqs[-1]], 0, k, v)
+        kept.append([ref.value8(*ref.quantize8(x[:, 0], G)) for x in (k, v)])
+    for starts, n in (([0, 0, 0], 77), ([63, 1, 255], 65), ([299, 76, 512], 1), ([10, 5, 500], 13)):
+        for out_dtype in (torch.float16, torch.bfloat16, torch.float32):
+            got = kb.read_rows(pool, seqs, 0, layers, n, starts=starts, dtype=out_dtype)
+            for i, at in enumerate(starts):
+                for x, y in zip(got, kept[i]):
+                    assert torch.equal(x[:, i], y[:, :, at:at + n].to(out_dtype))
+    win = kb.KVPool(1, hkv, 4, D, num_blocks=16, group_size=G, window=100, max_append=200)
+    seq = win.create_sequence()
+    for n in (200, 200, 130, 200):
+        k, v = (rows(g, (1, 1, hkv, n, D), dtype) for _ in range(2))
+        kb.append_quantize(win, [seq], 0, k, v)
+    got = kb.read_rows(win, [seq], 0, 1, 200, starts=[530])
+    for x, y in zip(got, (k, v)):
+        assert torch.equal(x[0, 0], ref.value8(*ref.quantize8(y[0, 0], G)).half())
+    pool.close()
+    win.close()
+
+
+@pytest.mark.parametrize("D,G,hq,hkv,nq,n", [(128, 64, 32, 8, 64, 700), (64, 64, 8, 2, 130, 207), (128, 128, 16, 16, 64, 64)])
+def test_prompt_path_against_the_format(D, G, hq, hkv, nq, n):
+    """Prompt chunks on tcgen05 take K and V rounded to f16, against the values
+    of the format. With |k| and |v| each off by 2^-11 at most, a query's scores
+    move by e = scale * max_t sum_d |q_d k_td| * 2^-11, its weights by a factor
+    exp(+-2e), its output by (exp(2e) - 1) spans of v; v itself adds 2^-11 of
+    its largest magnitude, and the f16 weights what tests/_int4.py bounds."""
+    scale = 1 / math.sqrt(D)
+    g = gen(n)
+    pool = pool4(1, hkv, hq, D, G)
+    seqs, kv = fill(pool, [n], torch.bfloat16, g, 1)
+    q = torch.randn(1, 1, nq, hq, D, device="cuda", generator=g).to(torch.bfloat16)
+    out = torch.empty(1, 1, nq, hq, D, device="cuda")
+    kb.prefill_attention(pool, seqs, 0, q, out, scale)
+    assert "umma" in pool.last_kernels()
+    k, v = kv[0][0][0], kv[0][1][0]
+    seen = (torch.arange(n, device="cuda")[None] <= (n - nq + torch.arange(nq, device="cuda"))[:, None])[:, None]
+    want = ref.attend(q[0, 0], k, v, scale, seen)
+    reach = torch.einsum("nhgd,htd->nhgt", q[0, 0].double().abs().reshape(nq, hkv, hq // hkv, D), k.abs()).amax(-1)
+    e = scale * reach.reshape(nq, hq, 1) * 2.0 ** -11
+    span = (v.amax() - v.amin()).item()
+    bound = torch.expm1(2 * e) * span + v.abs().max().item() * 2.0 ** -11 + ref.tolerance(2 * v, out.dtype, want)
+    err = (out[0, 0].double() - want).abs()
+    assert (err <= bound).all(), f"{err.max().item():.3e}"
     pool.close()
