@@ -94,6 +94,11 @@ enum {
  *   scale = f16(f32(max - min) / 15), zero = f16(min)
  *   code  = clip(round-half-even((x - zero) / scale), 0, 15), in f32 (scale 0: 0)
  *   value = code * scale + zero in f32
+ * Decode and verify attention compute on these values' parts; prompt chunks of
+ * 64 query rows (n_query times query heads per kv head) and more and the
+ * shared-prefix cascade (head_dim 64 and 128) take the values rounded to f16.
+ * At head_dim 256 a 4-bit pool has neither: a prompt chunk runs as verify
+ * units, forks of a prefix each read it for themselves.
  * Inputs beyond +-61440 saturate and NaN counts as 0, and of restored rows a
  * zero is kept within +-61440, a scale where all sixteen values are finite in
  * f16, NaN as 0, so a 4-bit cache never holds an infinity or NaN. Every call

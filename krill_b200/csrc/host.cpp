@@ -905,7 +905,9 @@ krill_status_t do_attention(krill_pool_t p, int32_t n_seqs, const krill_seq_t* s
       // its start and end, come out least. 24 runs of 512 sub-blocks over 148
       // CTAs: pieces of 16 make shares up to 1.16 times the mean, of 29 1.02;
       // decode at that size went from 122 to 107 us, 4 queries over 16 ragged
-      // sequences from 138 to 121.
+      // sequences from 138 to 121. (The other formats keep their pieces, and
+      // with them the order of their sums: their results stay bit for bit what
+      // they were before 4-bit pools.)
       const int step = qt2 ? 2 : 1;
       // layers of equal lengths are counted once
       const int64_t per_layer = n_units / lc;

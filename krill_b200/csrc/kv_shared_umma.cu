@@ -27,10 +27,11 @@
 // Causal items (verify, chunked prefill) write the rows they finish straight to
 // the output; only row blocks cut between two CTAs leave records.
 // 512 queries of 8 sequences behind 4096 tokens of a 4-bit pool, 2 layers, 32
-// heads over 8 of 128: 814 us, 0.44 of the bf16 peak. The softmax bounds it: per
-// tile of 128 x 64 scores the exponentials alone take 512 cycles for the 719 of
-// the tile's two products, and the chain S, softmax, P.V of one half of the rows
-// overlaps only the other half's.
+// heads over 8 of 128: 814 us, 0.44 of the bf16 peak. Latency bounds it, no unit
+// does: a tile of 128 x 64 scores takes 1520 cycles, in which the tensor core is
+// busy for 46 %, the exponentials' unit for 36 %, the ALU for 44 % and the issue
+// slots for 59 %. The chain S, softmax, P.V of one half of the rows overlaps
+// only the other half's.
 // Every wait is bounded (the pool's wait_timeout_us, then 20 us after the
 // first timeout) and sets the pool's error flag; the tensor memory is released
 // on every path.

@@ -183,3 +183,20 @@ def test_prompt_path_against_the_format(D, G, hq, hkv, nq, n):
     err = (out[0, 0].double() - want).abs()
     assert (err <= bound).all(), f"{err.max().item():.3e}"
     pool.close()
+
+
+@pytest.mark.parametrize("D,hq,hkv,split", [(128, 32, 8, 256), (64, 4, 2, 64), (256, 4, 2, 128)])
+def test_fixed_pieces_do_not_depend_on_the_batch(D, hq, hkv, split):
+    """With a fixed split_tokens a sequence's output is the same alone and in
+    a batch, bit for bit."""
+    lens, layers = [300, 900, 4000, 65], 2
+    g = gen(D + split)
+    pool = pool4(layers, hkv, hq, D, 64, split_tokens=split)
+    seqs, _ = fill(pool, lens, torch.bfloat16, g, layers)
+    q = torch.randn(layers, 4, hq, D, device="cuda", generator=g).to(torch.bfloat16)
+    out, one = torch.empty(layers, 4, hq, D, device="cuda"), torch.empty(layers, 1, hq, D, device="cuda")
+    kb.decode_attention(pool, seqs, 0, q, out, 0.09)
+    for i in range(4):
+        kb.decode_attention(pool, [seqs[i]], 0, q[:, i:i + 1].contiguous(), one, 0.09)
+        assert torch.equal(one[:, 0], out[:, i])
+    pool.close()
